@@ -10,6 +10,7 @@
 #ifndef GSR_OPTIM_H
 #define GSR_OPTIM_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -48,6 +49,34 @@ int gsr_adam_step_guarded(int n_tensors, float* const* params, const float* cons
                           const double* lr, const double* weight_decay, const double* step,
                           double beta1, double beta2, double eps, const float* skip,
                           uint32_t* host_skipped, void* stream);
+
+/* gsr_adam_step_guarded on gradients multiplied by *grad_scale (a device float written earlier on
+ * `stream`, e.g. by gsr_grad_norm; NULL = 1): clipping by the global norm without a pass of its own
+ * over the gradients, which stay as they are. */
+int gsr_adam_step_scaled(int n_tensors, float* const* params, const float* const* grads,
+                         float* const* exp_avg, float* const* exp_avg_sq, const int64_t* numel,
+                         const double* lr, const double* weight_decay, const double* step,
+                         double beta1, double beta2, double eps, const float* skip,
+                         uint32_t* host_skipped, const float* grad_scale, void* stream);
+
+/* The norm of all elements of n_tensors >= 1 gradients together (torch.nn.utils.clip_grad_norm_'s
+ * total norm).  grads[t]: device pointer to numel[t] (0 allowed) contiguous elements of dtype[t]
+ * (GSR_F32 / GSR_F16 / GSR_BF16, gsr_linear.h); sums are held in 64 bits.  norm: device float;
+ * scale (or NULL): device float receiving min(1, max_norm / (norm + 1e-6)), NaN if the norm is.
+ * Any number of tensors: GSR_CLIP_LAUNCH_TENSORS to a launch.  scratch: device memory of
+ * gsr_grad_norm_scratch_bytes(n_tensors) bytes, 8-byte aligned, holding nothing between calls.
+ * The same gradients give the same bits.  0 ok, 1 invalid arguments, 2 launch error. */
+enum { GSR_NORM_INF = 0, GSR_NORM_1 = 1, GSR_NORM_2 = 2 };
+#define GSR_CLIP_LAUNCH_TENSORS 128
+size_t gsr_grad_norm_scratch_bytes(int n_tensors);
+int gsr_grad_norm(int n_tensors, const void* const* grads, const int64_t* numel, const int* dtype,
+                  int norm_type, float max_norm, float* norm, float* scale, void* scratch,
+                  void* stream);
+
+/* gsr_grad_norm, then every gradient times scale in place, rounded once to its type (untouched
+ * when scale is 1).  max_norm >= 0.  The tensors must not overlap. */
+int gsr_clip_grads(int n_tensors, void* const* grads, const int64_t* numel, const int* dtype,
+                   int norm_type, float max_norm, float* norm, void* scratch, void* stream);
 
 #ifdef __cplusplus
 }

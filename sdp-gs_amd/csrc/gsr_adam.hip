@@ -52,6 +52,7 @@ struct AdamArgs {
   // NaN), so every parameter and moment stays untouched (include/gsr_optim.h)
   const float* skip;
   uint32_t* host_skipped;  // pinned host word: 1 = this step was skipped, 0 = applied (or NULL)
+  const float* grad_scale;  // the step's clipping factor (gsr_clip.hip), or NULL = 1
 };
 
 __device__ __forceinline__ float lerp_torch(float a, float b, float w) {
@@ -112,6 +113,8 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(AdamArgs a) {
   if (a.host_skipped && blockIdx.x == 0 && threadIdx.x == 0)
     __hip_atomic_store(a.host_skipped, skipped ? 1u : 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   if (skipped) return;
+  // a product with 1 is exact, so a step without clipping keeps its bits
+  const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
   const uint32_t b = blockIdx.x;
   int t = 0;
   while (t + 1 < a.n && b >= a.block0[t + 1]) t++;  // workgroup-uniform, <= 16 tensors
@@ -135,10 +138,10 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(AdamArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < kVecPerThread; u++) {
-      adam_one(pv[u].x, gv[u].x, mv[u].x, vv[u].x, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
-      adam_one(pv[u].y, gv[u].y, mv[u].y, vv[u].y, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
-      adam_one(pv[u].z, gv[u].z, mv[u].z, vv[u].z, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
-      adam_one(pv[u].w, gv[u].w, mv[u].w, vv[u].w, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
+      adam_one(pv[u].x, gv[u].x * gs, mv[u].x, vv[u].x, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
+      adam_one(pv[u].y, gv[u].y * gs, mv[u].y, vv[u].y, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
+      adam_one(pv[u].z, gv[u].z * gs, mv[u].z, vv[u].z, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
+      adam_one(pv[u].w, gv[u].w * gs, mv[u].w, vv[u].w, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
       const int64_t q = (base >> 2) + (int64_t)u * kThreads + threadIdx.x;
       st4<GSR_ADAM_NT >= 1>(reinterpret_cast<float4*>(P) + q, pv[u]);
       st4<GSR_ADAM_NT >= 1>(reinterpret_cast<float4*>(M) + q, mv[u]);
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(AdamArgs a) {
   const int64_t end = base + kBlockElems < n ? base + kBlockElems : n;
   for (int64_t i = base + threadIdx.x; i < end; i += kThreads) {
     float p = P[i], m = M[i], v = V[i];
-    adam_one(p, G[i], m, v, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
+    adam_one(p, G[i] * gs, m, v, wd, a.w1, a.beta2, a.one_m_beta2, a.eps, ss, bc);
     P[i] = p;
     M[i] = m;
     V[i] = v;
@@ -203,6 +206,18 @@ extern "C" int gsr_adam_step_guarded(int n_tensors, float* const* params, const 
                                      const double* weight_decay, const double* step, double beta1,
                                      double beta2, double eps, const float* skip,
                                      uint32_t* host_skipped, void* stream) {
+  return gsr_adam_step_scaled(n_tensors, params, grads, exp_avg, exp_avg_sq, numel, lr,
+                              weight_decay, step, beta1, beta2, eps, skip, host_skipped, nullptr,
+                              stream);
+}
+
+extern "C" int gsr_adam_step_scaled(int n_tensors, float* const* params, const float* const* grads,
+                                    float* const* exp_avg, float* const* exp_avg_sq,
+                                    const int64_t* numel, const double* lr,
+                                    const double* weight_decay, const double* step, double beta1,
+                                    double beta2, double eps, const float* skip,
+                                    uint32_t* host_skipped, const float* grad_scale,
+                                    void* stream) {
   if (n_tensors < 0 || n_tensors > GSR_ADAM_MAX_TENSORS) return 1;
   if (n_tensors == 0) return 0;
   AdamArgs a{};
@@ -241,6 +256,7 @@ extern "C" int gsr_adam_step_guarded(int n_tensors, float* const* params, const 
   }
   a.skip = skip;
   a.host_skipped = host_skipped;
+  a.grad_scale = grad_scale;
   hipLaunchKernelGGL(adam_kernel, dim3(blocks), dim3(kThreads), 0, (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }

@@ -219,6 +219,16 @@ def load():
             _p]                                          # stream
         L.gsr_adam_step_guarded.restype = _i
         L.gsr_adam_step_guarded.argtypes = list(L.gsr_adam_step.argtypes[:-1]) + [_p, _p, _p]
+        L.gsr_adam_step_scaled.restype = _i
+        L.gsr_adam_step_scaled.argtypes = list(L.gsr_adam_step.argtypes[:-1]) + [_p, _p, _p, _p]
+        L.gsr_grad_norm_scratch_bytes.restype = _sz
+        L.gsr_grad_norm_scratch_bytes.argtypes = [_i]
+        L.gsr_grad_norm.restype = _i
+        L.gsr_grad_norm.argtypes = [_i, _pp, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(_i),
+                                    _i, _f, _p, _p, _p, _p]
+        L.gsr_clip_grads.restype = _i
+        L.gsr_clip_grads.argtypes = [_i, _pp, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(_i),
+                                     _i, _f, _p, _p, _p]
         L.gsr_step_guard.restype = _i
         L.gsr_step_guard.argtypes = [_p, _p]
         # include/gsr_densify.h
@@ -265,6 +275,23 @@ def load():
         L.gsr_view_loss_views_backward.restype = _i
         L.gsr_view_loss_views_backward.argtypes = [_i, _i, _i, _i, _p, _p, _f, _i64, _p, _p, _f,
                                                    _f, _p, _p, _p, _p, _p]
+        # include/gsr_linear.h
+        L.gsr_linear.restype = _i
+        L.gsr_linear.argtypes = [_i, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i,
+                                 _p, _i64, _p]
+        L.gsr_linear_backward_scratch_bytes.restype = _sz
+        L.gsr_linear_backward_scratch_bytes.argtypes = [_i, _i64, _i64, _i64, _i, _i]
+        L.gsr_linear_backward.restype = _i
+        L.gsr_linear_backward.argtypes = [_i, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i,
+                                          _p, _i64, _p, _p, _p, _p, _p]
+        L.gsr_gated.restype = _i
+        L.gsr_gated.argtypes = [_i, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i, _p, _i64,
+                                _p]
+        L.gsr_gated_backward_scratch_bytes.restype = _sz
+        L.gsr_gated_backward_scratch_bytes.argtypes = [_i, _i64, _i64, _i64, _i]
+        L.gsr_gated_backward.restype = _i
+        L.gsr_gated_backward.argtypes = [_i, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i,
+                                         _p, _i64, _p, _p, _p, _p, _p]
         # include/gsr_knn.h
         L.gsr_knn_scratch_bytes.restype = _sz
         L.gsr_knn_scratch_bytes.argtypes = [_i64]

@@ -1,0 +1,205 @@
+"""Fused matrix products on libgsr (include/gsr_linear.h): what a feature head is made of.
+
+  fused_linear(x, weight, bias, activation=, residual=)   act(x W^T + b) + r
+  gated_linear(x, gate_weight, up_weight, gate_bias, up_bias, activation=)
+                                                act(x Wg^T + bg) * (x Wu^T + bu)
+
+Each forward is ONE launch, with bias, activation and residual (or the product of the two halves)
+in the matrix product's epilogue.  The backward keeps nothing but the inputs: it forms the
+pre-activations again, in 32 bits, in the product that writes their gradients -- cheaper than
+storing and reading them back at a head's widths, and free of their rounding.  float32, float16
+and bfloat16 (one type per call); sums and activations in 32 bits, every result rounded once.
+Results do not depend on timing.  No CPU path.
+
+A rendered feature image [C,H,W] goes in as it lies: ``fused_linear(image.reshape(C, -1).t(), W)``
+reads the channel-major memory in place.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}  # GSR_ACT_*; gelu is the erf form
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # GSR_F32 / F16 / BF16
+
+
+def _check(rc, what):
+    if rc != 0:
+        raise RuntimeError(f"{what} failed with status {rc}")
+
+
+def _checked(x, others, activation):
+    """Refuse what the kernels do not take (before any GPU work)."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
+    for name, t, shape in others:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+        if t.dtype != x.dtype:
+            raise ValueError(f"{name} must have x's type {x.dtype}, not {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"{name} must be on x's device {x.device}, not {t.device}")
+    if x.dtype not in DTYPES:
+        raise ValueError(f"float32, float16 or bfloat16 expected, not {x.dtype}")
+    if not x.is_cuda:
+        raise RuntimeError("gsr fused products run on HIP tensors only (no CPU path)")
+
+
+def _weight_sizes(x, weight, name):
+    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
+        raise TypeError(f"x and {name} must be tensors")
+    if x.dim() < 1 or weight.dim() != 2:
+        raise ValueError(f"x must be [..., K] and {name} [N, K]")
+    N, K = (int(n) for n in weight.shape)
+    if N < 1 or K < 1:
+        raise ValueError(f"{name} [N, K] must not be empty")
+    return N, K
+
+
+def _rows(t, n):
+    """t [..., n] as a [M, n] matrix whose rows are contiguous (a copy only if it has to be)."""
+    t = t.detach()
+    m = t.reshape(-1, n) if t.dim() != 2 else t
+    if (n > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < n):
+        m = m.contiguous()
+    return m
+
+
+def _row_stride(m):
+    """The distance between rows (a single row's stride means nothing)."""
+    return int(m.stride(0)) if m.shape[0] > 1 else int(m.shape[1])
+
+
+def _x_matrix(x, K):
+    """x as (matrix, row stride, column stride): channel-major memory is taken as it lies."""
+    x = x.detach()
+    if x.dim() == 2 and K > 1 and x.shape[0] > 1 and x.stride(0) == 1 and x.stride(1) >= x.shape[0]:
+        return x, 1, int(x.stride(1))
+    m = _rows(x, K)
+    return m, _row_stride(m), 1
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _scratch(nbytes, device):
+    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        N, K = weight.shape
+        xm, x_row, x_col = _x_matrix(x, K)
+        M = xm.shape[0]
+        w = _rows(weight, K)
+        b = None if bias is None else bias.detach().contiguous()
+        r = None if residual is None else _rows(residual, N)
+        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        if M:
+            with _lib.on_device(x.device):
+                _check(_lib.load().gsr_linear(
+                    DTYPES[x.dtype], M, K, N, xm.data_ptr(), x_row, x_col, w.data_ptr(),
+                    _row_stride(w), _ptr(b), _ptr(r), 0 if r is None else _row_stride(r), act,
+                    y.data_ptr(), N, _lib.raw_stream(x.device)), "gsr_linear")
+        ctx.save_for_backward(xm, w, b)
+        ctx.args = (x.shape, x_row, x_col, act)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xm, w, b = ctx.saved_tensors
+        shape, x_row, x_col, act = ctx.args
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        (N, K), M = w.shape, xm.shape[0]
+        kind, dev = xm.dtype, xm.device
+        dx = torch.empty(shape, dtype=kind, device=dev) if need_x else None
+        dw = torch.empty((N, K), dtype=kind, device=dev) if need_w else None
+        db = torch.empty(N, dtype=kind, device=dev) if need_b else None
+        if need_x or need_w or need_b:
+            g = _rows(dy, N)
+            L = _lib.load()
+            scratch = _scratch(L.gsr_linear_backward_scratch_bytes(
+                DTYPES[kind], M, K, N, act, int(need_w or need_b)), dev)
+            with _lib.on_device(dev):
+                _check(L.gsr_linear_backward(
+                    DTYPES[kind], M, K, N, xm.data_ptr(), x_row, x_col, w.data_ptr(),
+                    _row_stride(w), _ptr(b), act, g.data_ptr(), _row_stride(g), _ptr(dx), _ptr(dw),
+                    _ptr(db), scratch.data_ptr(), _lib.raw_stream(dev)), "gsr_linear_backward")
+        return dx, dw, db, dy if need_r else None, None
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, gate_bias, up_bias, act):
+        N, K = gate.shape
+        xm = _rows(x, K)
+        M = xm.shape[0]
+        wg, wu = _rows(gate, K), _rows(up, K)
+        if _row_stride(wg) != _row_stride(wu):
+            wg, wu = wg.contiguous(), wu.contiguous()
+        bg = None if gate_bias is None else gate_bias.detach().contiguous()
+        bu = None if up_bias is None else up_bias.detach().contiguous()
+        h = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        if M:
+            with _lib.on_device(x.device):
+                _check(_lib.load().gsr_gated(
+                    DTYPES[x.dtype], M, K, N, xm.data_ptr(), _row_stride(xm), wg.data_ptr(),
+                    wu.data_ptr(), _row_stride(wg), _ptr(bg), _ptr(bu), act, h.data_ptr(), N,
+                    _lib.raw_stream(x.device)), "gsr_gated")
+        ctx.save_for_backward(xm, wg, wu, bg, bu)
+        ctx.args = (x.shape, act)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        xm, wg, wu, bg, bu = ctx.saved_tensors
+        shape, act = ctx.args
+        need = ctx.needs_input_grad
+        (N, K), M = wg.shape, xm.shape[0]
+        kind, dev = xm.dtype, xm.device
+        need_w, need_b = need[1] or need[2], need[3] or need[4]
+        dx = torch.empty(shape, dtype=kind, device=dev) if need[0] else None
+        dw = torch.empty((2, N, K), dtype=kind, device=dev) if need_w else None
+        db = torch.empty((2, N), dtype=kind, device=dev) if need_b else None
+        if need[0] or need_w or need_b:
+            g = _rows(dh, N)
+            L = _lib.load()
+            scratch = _scratch(L.gsr_gated_backward_scratch_bytes(
+                DTYPES[kind], M, K, N, int(need_w or need_b)), dev)
+            with _lib.on_device(dev):
+                _check(L.gsr_gated_backward(
+                    DTYPES[kind], M, K, N, xm.data_ptr(), _row_stride(xm), wg.data_ptr(),
+                    wu.data_ptr(), _row_stride(wg), _ptr(bg), _ptr(bu), act, g.data_ptr(),
+                    _row_stride(g), _ptr(dx), _ptr(dw), _ptr(db), scratch.data_ptr(),
+                    _lib.raw_stream(dev)), "gsr_gated_backward")
+        return (dx, dw[0] if need[1] else None, dw[1] if need[2] else None,
+                db[0] if need[3] else None, db[1] if need[4] else None, None)
+
+
+def fused_linear(x, weight, bias=None, *, activation="none", residual=None):
+    """activation(x @ weight.T + bias) + residual.  x [..., K], weight [N, K], bias [N], residual
+    [..., N] (the result's shape); differentiable once in each of them."""
+    N, K = _weight_sizes(x, weight, "weight")
+    _checked(x, [("x", x, x.shape[:-1] + (K,)), ("weight", weight, (N, K)), ("bias", bias, (N,)),
+                 ("residual", residual, x.shape[:-1] + (N,))], activation)
+    return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation])
+
+
+def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, activation="silu"):
+    """activation(x @ gate_weight.T + gate_bias) * (x @ up_weight.T + up_bias), both products in
+    one pass over x.  x [..., K], weights [N, K], biases [N]; differentiable once in each."""
+    N, K = _weight_sizes(x, gate_weight, "gate_weight")
+    _checked(x, [("x", x, x.shape[:-1] + (K,)), ("gate_weight", gate_weight, (N, K)),
+                 ("up_weight", up_weight, (N, K)), ("gate_bias", gate_bias, (N,)),
+                 ("up_bias", up_bias, (N,))], activation)
+    return _Gated.apply(x, gate_weight, up_weight, gate_bias, up_bias, ACTIVATIONS[activation])

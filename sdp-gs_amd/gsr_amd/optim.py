@@ -16,10 +16,15 @@ next step() reads it (no synchronisation in the normal case) and, for a skipped 
 the step counts it had advanced (state["step"]: a skipped step leaves parameters, moments AND
 counts as they were) and raises, unless reset_forward_faults() ran since the skipped step -- a
 caller that swallows one error does not silently stall.
+
+Gradient clipping: `grad_norm` and `clip_grad_norm_` (torch.nn.utils' total norm and in-place
+scaling, one streaming pass each over any number of tensors of mixed types), and
+``FusedAdam(..., max_grad_norm=)``, which applies the same factor inside the Adam launch.
 """
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -27,18 +32,154 @@ from . import _lib
 
 MAX_TENSORS = 16  # GSR_ADAM_MAX_TENSORS
 
+_NORMS = {math.inf: 0, 1.0: 1, 2.0: 2}  # GSR_NORM_INF / 1 / 2
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # GSR_F32 / F16 / BF16
+
+
+def _dense(t):
+    """Whether t's elements fill its memory without gaps or repeats, in any order of dimensions
+    (then the kernels take them in the order they lie)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1),
+                               key=lambda d: d[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _norm_args(tensors, norm_type):
+    """The tensors that hold elements, checked: (tensors, norm code)."""
+    if isinstance(norm_type, str) or float(norm_type) not in _NORMS:
+        raise ValueError(f"norm_type must be 1, 2 or inf, not {norm_type!r}")
+    kept = []
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise RuntimeError("gradient norm: sparse gradients are not supported")
+        if t.dtype not in _DTYPES:
+            raise ValueError(f"gradient norm: float32, float16 or bfloat16 expected, not {t.dtype}")
+        if not t.is_cuda:
+            raise RuntimeError("gradient norm: HIP tensors only (no CPU path)")
+        if t.device != tensors[0].device:
+            raise ValueError("gradient norm: every gradient must be on one device")
+        if t.numel():
+            kept.append(t)
+    return kept, _NORMS[float(norm_type)]
+
+
+def _c_tensors(ts):
+    n = len(ts)
+    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]),
+            (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
+            (ctypes.c_int * n)(*[_DTYPES[t.dtype] for t in ts]))
+
+
+def _norm_and_scale(tensors, norm_code, max_norm, scale=None):
+    """gsr_grad_norm on the current stream: the norm (and `scale`, a one-float tensor)."""
+    dev = tensors[0].device
+    ts = [t.detach() if _dense(t) else t.detach().contiguous() for t in tensors]
+    ptrs, numel, kinds = _c_tensors(ts)
+    L = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    scratch = torch.empty(int(L.gsr_grad_norm_scratch_bytes(len(ts))), dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        rc = L.gsr_grad_norm(len(ts), ptrs, numel, kinds, norm_code, float(max_norm),
+                             norm.data_ptr(), None if scale is None else scale.data_ptr(),
+                             scratch.data_ptr(), _lib.raw_stream(dev))
+    if rc != 0:
+        raise RuntimeError(f"gsr_grad_norm failed with status {rc}")
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(tensors, norm_type=2.0):
+    """The norm (1, 2 or inf) of all elements of `tensors` together, as a float32 scalar on their
+    device (not synchronised).  Any number of tensors, of mixed types, strides and sizes; sums in
+    64 bits, the same tensors give the same bits.  No tensors (or only empty ones): 0."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    kept, code = _norm_args(tensors, norm_type)
+    if not kept:
+        return torch.zeros((), device=tensors[0].device if tensors else "cpu")
+    return _norm_and_scale(kept, code, math.inf)
+
+
+def _refuse_overlap(grads):
+    """Two workgroups may not scale the same memory.  Gradients with gaps are scaled in copies, so
+    only their overlap with one that is scaled in place counts."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(
+        (n - 1) * s for n, s in zip(t.shape, t.stride()))), _dense(t)) for t in grads)
+    end_dense = end_any = 0
+    for start, end, dense in spans:
+        if start < (end_any if dense else end_dense):
+            raise ValueError("clip_grad_norm_: two gradients share memory (the same one twice?)")
+        end_any = max(end_any, end)
+        if dense:
+            end_dense = max(end_dense, end)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_: scale every parameter's .grad in place by
+    min(1, max_norm / (norm + 1e-6)), norm = grad_norm of all of them; returns the norm.  As there,
+    a norm that is NaN makes every gradient NaN, unless error_if_nonfinite (which waits for the
+    norm) raises first.  Gradients must not share memory with each other."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be at least 0, not {max_norm}")
+    grads = [p.grad for p in parameters if p.grad is not None]
+    kept, code = _norm_args(grads, norm_type)
+    if not kept:
+        return torch.zeros((), device=grads[0].device if grads else "cpu")
+    for t in kept:
+        if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+            raise ValueError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
+    _refuse_overlap(kept)
+    if error_if_nonfinite:
+        norm = _norm_and_scale(kept, code, math.inf)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"The total norm of order {norm_type} is non-finite, so it cannot "
+                               "be clipped")
+    dev = kept[0].device
+    ts = [t.detach() if _dense(t) else t.detach().contiguous() for t in kept]
+    ptrs, numel, kinds = _c_tensors(ts)
+    L = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    scratch = torch.empty(int(L.gsr_grad_norm_scratch_bytes(len(ts))), dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        rc = L.gsr_clip_grads(len(ts), ptrs, numel, kinds, code, max_norm, norm.data_ptr(),
+                              scratch.data_ptr(), _lib.raw_stream(dev))
+    if rc != 0:
+        raise RuntimeError(f"gsr_clip_grads failed with status {rc}")
+    for t, c in zip(kept, ts):
+        if t.data_ptr() != c.data_ptr():  # a gradient with gaps: its scaled copy goes back
+            t.copy_(c)
+    return norm
+
 
 class FusedAdam(torch.optim.Adam):
+    """max_grad_norm: clip by the global 2-norm of every parameter's gradient in each step, as
+    clip_grad_norm_(parameters, max_grad_norm) before it would, but inside the Adam launch: .grad
+    keeps its unclipped values.  `grad_norm` is the last step's norm (a device scalar, not
+    synchronised; None before the first step or without max_grad_norm).  A step in row slices
+    (begin_rows) takes the norm when it begins, so every gradient must be final by then."""
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
-                 amsgrad=False, *, maximize=False):
+                 amsgrad=False, *, maximize=False, max_grad_norm=None):
         if amsgrad or maximize:
             raise ValueError("FusedAdam implements Adam without amsgrad / maximize")
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError(f"max_grad_norm must be at least 0, not {max_grad_norm}")
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                          amsgrad=False, foreach=False)
         self._mailbox = {}     # device -> pinned int32 [1]: 1 = the step's launches skipped it
         self._guard = {}       # device -> float32 [1] device slot: the step's one fault snapshot
         self._pending = None   # (events, mailboxes, stepped states, fault-reset count)
         self.skipped_steps = 0
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
 
     def _resolve_pending(self):
         """The previous step's device decision: undo its step counts if it was skipped."""
@@ -85,6 +226,10 @@ class FusedAdam(torch.optim.Adam):
         parameter (dim 0), end_rows(h) finishes.  The row ranges must cover every row exactly
         once; the result is bitwise the one of step() (the update is elementwise)."""
         self._resolve_pending()
+        kept, norm_code = [], 2
+        if self.max_grad_norm is not None:  # refused before any step count advances
+            kept, norm_code = _norm_args([p.grad for group in self.param_groups
+                                          for p in group["params"] if p.grad is not None], 2.0)
         batches = {}
         for group in self.param_groups:
             beta1, beta2 = group["betas"]
@@ -138,7 +283,12 @@ class FusedAdam(torch.optim.Adam):
             else:
                 skips[dev] = (skip.data_ptr(), box)
         states = [self.state[it[0]] for its in batches.values() for it in its]
-        return {"batches": batches, "skips": skips, "states": states, "issued": False}
+        scale = None
+        if kept:
+            scale = torch.empty(1, dtype=torch.float32, device=kept[0].device)
+            self.grad_norm = _norm_and_scale(kept, norm_code, self.max_grad_norm, scale)
+        return {"batches": batches, "skips": skips, "states": states, "issued": False,
+                "scale": scale}
 
     def abort_rows(self, h):
         """Give back the step counts begin_rows advanced when the step is abandoned before any
@@ -157,6 +307,10 @@ class FusedAdam(torch.optim.Adam):
         Issued on the current stream of each parameter's device."""
         L = _lib.load()
         h["issued"] = True
+        scale = None
+        if h["scale"] is not None:
+            scale = h["scale"].data_ptr()
+            h["scale"].record_stream(torch.cuda.current_stream(h["scale"].device))
         for (dev, beta1, beta2, eps), items in h["batches"].items():
             stream = _lib.raw_stream(dev)
             skip_ptr, box = h["skips"][dev]
@@ -177,9 +331,9 @@ class FusedAdam(torch.optim.Adam):
                 wd = (ctypes.c_double * n)(*[s[0][5] for s in chunk])
                 steps = (ctypes.c_double * n)(*[s[0][6] for s in chunk])
                 with _lib.on_device(dev):
-                    rc = L.gsr_adam_step_guarded(n, ptrs[0], ptrs[1], ptrs[2], ptrs[3], numel, lr,
-                                                 wd, steps, beta1, beta2, eps, skip_ptr,
-                                                 box.data_ptr(), stream)
+                    rc = L.gsr_adam_step_scaled(n, ptrs[0], ptrs[1], ptrs[2], ptrs[3], numel, lr,
+                                                wd, steps, beta1, beta2, eps, skip_ptr,
+                                                box.data_ptr(), scale, stream)
                 if rc != 0:
                     raise RuntimeError(f"gsr_adam_step failed with status {rc}")
 

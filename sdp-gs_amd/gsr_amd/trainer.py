@@ -13,7 +13,9 @@
 The language-feature loss (loss_feature_metric) and the pseudo-view branch (:101-193) need the
 scene's CLIP features / MiDaS depth, which a synthetic benchmark does not have; the feature image is
 still rendered (include_feature) and the pseudo-view interval is past end_sample_pseudo at the
-reference's defaults for most of training.  `train_step_views` is the batched multi-view form of the
+reference's defaults for most of training.  Given a feature head and wide target features,
+train_iteration trains both through the rendered feature image; with args.max_grad_norm every step's
+gradients are clipped by their global norm.  `train_step_views` is the batched multi-view form of the
 same iteration (ViewPipeline over HIP streams, gradients summed over the views, one optimizer step;
 with a GradAllReducer the per-view gradients of all ranks are summed first).
 """
@@ -43,6 +45,10 @@ class OptArgs:
     prune_threshold: float = 0.01
     depth_weight: float = 0.05
     include_feature: bool = True
+    # beyond the reference: the weight of the feature head's loss, and clipping of the step's
+    # gradients by their global 2-norm (None = off)
+    feature_weight: float = 1.0
+    max_grad_norm: Optional[float] = None
 
 
 class _Pipe:  # PipelineParams defaults (arguments/__init__.py:66-72)
@@ -88,25 +94,58 @@ def _guard_step():
     dgr.check_forwards(wait=False)
 
 
-def _optimizer_step(model, reducer=None):
+def _optimizer_step(model, reducer=None, args=None, head=None):
     """optimizer.step(); with a multi-GPU reducer FusedAdam takes the ranks' summed fault
-    snapshot as its skip decision (any rank failed -> every rank skips)."""
-    from .optim import FusedAdam
+    snapshot as its skip decision (any rank failed -> every rank skips).
+    args.max_grad_norm: the gradients clipped by their global norm -- inside the Adam launch, or,
+    where a head's are part of the norm (or the optimizer is another), in place before it."""
+    from . import _lib
+    from .optim import FusedAdam, clip_grad_norm_
     opt = model.optimizer
+    limit = None if args is None else getattr(args, "max_grad_norm", None)
     skip = reducer.skip_flag() if reducer is not None else None
+    if limit is not None and (head is not None or not isinstance(opt, FusedAdam)):
+        clip_grad_norm_([p for g in opt.param_groups for p in g["params"]]
+                        + ([] if head is None else list(head.parameters())), limit)
+        limit = None
+    if head is not None:
+        if skip is None:  # one snapshot for both optimizers: both step or neither does
+            skip = torch.empty(1, dtype=torch.float32, device=model.get_xyz.device)
+            _lib.step_guard(skip)
+        head.optimizer.step(skip=skip)
     if isinstance(opt, FusedAdam):
-        opt.step(skip=skip)
+        own = opt.max_grad_norm
+        if limit is not None:
+            opt.max_grad_norm = limit
+        try:
+            opt.step(skip=skip)
+        finally:
+            opt.max_grad_norm = own
     else:
         opt.step()
 
 
+def feature_loss(decoded, target):
+    """1 - the mean cosine between decoded and target features [..., D]."""
+    return 1.0 - torch.nn.functional.cosine_similarity(decoded.float(), target.float(),
+                                                       dim=-1).mean()
+
+
 def train_iteration(model, cam, gt_image, depth_mono, bg, args: OptArgs, iteration: int,
-                    extent: float, pipe=None):
-    """One reference iteration on one camera.  Returns the loss tensor (not synchronised)."""
+                    extent: float, pipe=None, feature_head=None, gt_feature=None):
+    """One reference iteration on one camera.  Returns the loss tensor (not synchronised).
+    feature_head (gsr_amd.feature_head.FeatureHead with its training_setup done) and gt_feature,
+    the wide features it should give: [H,W,D], or ([S,D], pixels [S]) for some pixels only.  The
+    loss gains args.feature_weight times feature_loss, and the head takes its own Adam step."""
     from gaussian_renderer import render
+    if (feature_head is None) != (gt_feature is None):
+        raise ValueError("train_iteration: feature_head and gt_feature belong together")
     pipe = pipe or _Pipe()
     pkg = render(cam, model, pipe, bg, args)
     loss = _view_loss(pkg, gt_image, depth_mono, args)
+    if feature_head is not None:
+        target, pixels = gt_feature if isinstance(gt_feature, tuple) else (gt_feature, None)
+        loss = loss + args.feature_weight * feature_loss(feature_head(pkg["feature"], pixels), target)
     loss.backward()
     with torch.no_grad():
         if iteration < args.densify_until_iter:
@@ -115,8 +154,10 @@ def train_iteration(model, cam, gt_image, depth_mono, bg, args: OptArgs, iterati
             if _densify_due(iteration, args):
                 densify_step(model, args, iteration, extent)
         _guard_step()
-        _optimizer_step(model)
+        _optimizer_step(model, args=args, head=feature_head)
         model.optimizer.zero_grad(set_to_none=True)
+        if feature_head is not None:
+            feature_head.optimizer.zero_grad(set_to_none=True)
     return loss.detach()
 
 
@@ -181,7 +222,9 @@ def train_step_views(model, cams: Sequence, gt_images: Sequence[torch.Tensor],
         opt = model.optimizer
         h = None
         if (reducer is not None and isinstance(opt, FusedAdam) and reducer._active()
-                and not reducer.average and not _densify_due(iteration, args)):
+                and not reducer.average and not _densify_due(iteration, args)
+                # a clipped step needs every gradient's norm before its first row
+                and getattr(args, "max_grad_norm", None) is None and opt.max_grad_norm is None):
             reducer.begin()  # the step's layout (also re-read by run_views)
             h = opt.begin_rows(skip=reducer.guard)
             fill = None
@@ -213,7 +256,7 @@ def train_step_views(model, cams: Sequence, gt_images: Sequence[torch.Tensor],
                                                model.max_radii2D)
                 densify_step(model, args, iteration, extent, generator=generator)
             _guard_step()
-            _optimizer_step(model, reducer)
+            _optimizer_step(model, reducer, args)
         return losses
 
     def forward(cam):
@@ -240,5 +283,5 @@ def train_step_views(model, cams: Sequence, gt_images: Sequence[torch.Tensor],
         # after a densification the new parameters have no .grad: Adam skips them, as in the
         # reference (train.py:223-231)
         _guard_step()
-        _optimizer_step(model, reducer)
+        _optimizer_step(model, reducer, args)
     return losses
