@@ -1,0 +1,6 @@
+// gsr_linear_bf16.hip -- the bfloat16 products of gsr_linear.hip (gsr_product.h).
+#include "gsr_product.h"
+
+namespace gsr {
+GSR_PRODUCTS(__hip_bfloat16)
+}

@@ -1,0 +1,6 @@
+// gsr_linear_f16.hip -- the 16-bit-float products of gsr_linear.hip (gsr_product.h).
+#include "gsr_product.h"
+
+namespace gsr {
+GSR_PRODUCTS(__half)
+}

@@ -1,0 +1,506 @@
+// gsr_product.h -- the tiled matrix-core product behind gsr_linear*.hip.
+//
+//   C(i, j) = sum_r A(i, r) B(j, r), one BI x BJ tile of C per workgroup, epilogues in gsr_linear.h.
+//
+// Matrix instruction: v_mfma_f32_16x16x32 on 16-bit operands, the rows of B (outputs j) as the
+// instruction's rows and the rows of A (i) as its columns, so that a lane's four results are four
+// consecutive j of one i and leave as 16-byte stores.
+//
+// 32-bit operands: a float is the exact sum of three bfloat16 parts (8 + 8 + 8 bits, each the
+// rounded remainder of the one before).  Six of the nine products of parts are formed, those of
+// 2^-16 or more; the three left out are below 2^-24 of the product together, a float product's own
+// rounding.  At 6/16 the rate of the 16-bit instruction that is 2.6x the float instruction's rate.
+// Parts of an infinity or a NaN do not sum to it, so a result that is not finite is computed again
+// from the operands in plain 32-bit arithmetic (exact_sum).
+//
+// LDS holds the operands' 16-bit planes.  An operand that is contiguous along r is kept as rows of
+// r and read 16 bytes (8 r) at a time; one that is contiguous along its rows is kept as it lies and
+// read through ds_read_b64_tr, which hands each lane 4 r of its own row.  16-byte chunks are
+// permuted within a row (swizzle) so that the 16 lanes of a read hit 16 different bank groups.
+#pragma once
+#include "gsr_linear.h"
+
+namespace gsr {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes at any address: operands may start anywhere (a slice, an odd row length)
+struct __attribute__((packed, aligned(1))) Bytes16 { u32x4 v; };
+
+template <typename T> struct Operand {
+  static constexpr int kPlanes = 1, kDepth = 64, kBuffers = 2, kRaw = 1;  // kRaw: 16-byte words per 8 elements
+};
+template <> struct Operand<float> {
+  static constexpr int kPlanes = 3, kDepth = 32, kBuffers = 1, kRaw = 2;
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mfma<__half>(s16x8 a, s16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t round_pair(f32x2 v) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+__device__ __forceinline__ f32x2 widen_pair(uint32_t v) {
+  return f32x2{__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)};
+}
+
+// 8 consecutive elements as they come from memory.
+template <typename T> struct Chunk {
+  u32x4 w[Operand<T>::kRaw];
+};
+
+// n of the 8 elements at p exist (n <= 0: none); the others are zero.
+template <typename T, bool FULL>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* p, int64_t n) {
+  Chunk<T> c;
+  if (FULL || n >= 8) {
+#pragma unroll
+    for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = ((const Bytes16*)p)[k].v;
+    return c;
+  }
+#pragma unroll
+  for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = u32x4{0, 0, 0, 0};
+  if (n <= 0) return c;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 7; e++)
+      if (e < n) c.w[e >> 2][e & 3] = ((const uint32_t*)p)[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; e++)
+      if (e < n) c.w[0][e >> 1] |= (uint32_t)((const uint16_t*)p)[e] << (16 * (e & 1));
+  }
+  return c;
+}
+
+// One operand's tile in LDS.  RC: contiguous along r (rows of kDepth), else rows of ROWS.
+// PAIRED: the epilogue takes 8 consecutive rows j per lane, so the 16 rows of a read are
+// 4 + 4 + 4 + 4 rows, 8 apart.
+template <typename T, bool RC, int ROWS, int THREADS, bool PAIRED>
+struct Tile {
+  static constexpr int kDepth = Operand<T>::kDepth, kPlanes = Operand<T>::kPlanes;
+  static constexpr int kPerRow = (RC ? kDepth : ROWS) / 8;   // chunks in a row of LDS
+  static constexpr int kChunks = ROWS * kDepth / 8 / THREADS;  // chunks a thread stages
+  static constexpr int kPlaneBytes = ROWS * kDepth * 2;
+  static constexpr int kBytes = kPlaneBytes * kPlanes;
+  static_assert(ROWS * kDepth % (8 * THREADS) == 0, "");
+
+  // Which of a row's chunks is kept where: the rows that one read takes together differ in it.
+  static __device__ __forceinline__ int swizzle(int row) {
+    if (!RC) {  // rows are r: a read takes 4 of each 8
+      if (ROWS == 64) return 2 * (((row >> 1) & 1) | (((row >> 3) & 1) << 1));
+      return 2 * ((row & 3) | (((row >> 3) & 1) << 2));
+    }
+    if (kDepth == 32) return (row >> 2) & 3;
+    return PAIRED ? ((row >> 1) & 1) | (((row >> 3) & 3) << 1) : (row >> 1) & 7;
+  }
+
+  // Rows [o0, o0 + ROWS) of O, r in [r0, r0 + kDepth) below r_end.  base1: rows from SPLIT on.
+  template <bool FULL, int SPLIT>
+  static __device__ __forceinline__ void load(Chunk<T> (&c)[kChunks], const T* base, const T* base1,
+                                              int64_t ld, int64_t o0, int64_t O, int64_t r0, int64_t r_end) {
+#pragma unroll
+    for (int s = 0; s < kChunks; s++) {
+      const int q = s * THREADS + threadIdx.x, row = q / kPerRow, col = q % kPerRow * 8;
+      if (RC) {
+        const bool second = SPLIT && row >= SPLIT;
+        const int64_t o = o0 + (second ? row - SPLIT : row);
+        const T* b = second ? base1 : base;
+        if (FULL) c[s] = load_chunk<T, true>(b + o * ld + r0 + col, 8);
+        else c[s] = load_chunk<T, false>(b + o * ld + r0 + col, o < O ? r_end - r0 - col : 0);
+      } else {
+        const T* p = base + (r0 + row) * ld + o0 + col;
+        if (FULL) c[s] = load_chunk<T, true>(p, 8);
+        else c[s] = load_chunk<T, false>(p, r0 + row < r_end ? O - o0 - col : 0);
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void store(char* lds, const Chunk<T> (&c)[kChunks]) {
+#pragma unroll
+    for (int s = 0; s < kChunks; s++) {
+      const int q = s * THREADS + threadIdx.x, row = q / kPerRow, at = q % kPerRow ^ swizzle(row);
+      u32x4* to = (u32x4*)(lds + (row * kPerRow + at) * 16);
+      if constexpr (kPlanes == 1) {
+        *to = c[s].w[0];
+      } else {
+        u32x4 part[3];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          f32x2 v = {__uint_as_float(c[s].w[k >> 1][(k & 1) * 2]), __uint_as_float(c[s].w[k >> 1][(k & 1) * 2 + 1])};
+#pragma unroll
+          for (int p = 0; p < 3; p++) {
+            part[p][k] = round_pair(v);
+            v -= widen_pair(part[p][k]);
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < 3; p++) *(u32x4*)((char*)to + p * kPlaneBytes) = part[p];
+      }
+    }
+  }
+
+  // The 16 rows of step t (of 16 rows each) and r in [32 kk, 32 kk + 32) as a matrix operand: lane
+  // l holds row l % 16 and r = 8 (l / 16) + 0..7.
+  static __device__ __forceinline__ s16x8 read(const char* lds, int t, int kk) {
+    const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+    if (RC) {
+      const int row = PAIRED ? 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3) : 16 * t + m;
+      return *(const s16x8*)(lds + row * (kPerRow * 16) + (((kk * 4 + q) ^ swizzle(row)) * 16));
+    }
+    const int p = m & 3, r = kk * 32 + 8 * q + (m >> 2);
+    const int col = PAIRED ? 32 * (t >> 1) + 8 * p + 4 * (t & 1) : 16 * t + 4 * p;
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds4*)(lds + r * (kPerRow * 16) + (((col >> 3) ^ swizzle(r)) * 16) + ((col >> 2) & 1) * 8));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds4*)(lds + (r + 4) * (kPerRow * 16) + (((col >> 3) ^ swizzle(r + 4)) * 16) + ((col >> 2) & 1) * 8));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// RUN consecutive elements of a row as floats; `n` of them exist.
+template <typename T, int RUN>
+__device__ __forceinline__ void load_run(float (&v)[RUN], const T* p, int64_t n) {
+  if (n >= RUN) {
+    const u32x4 w = ((const Bytes16*)p)->v;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < RUN; k++) v[k] = __uint_as_float(w[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < RUN; k++) {
+        const uint16_t b = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+        v[k] = to_f(__builtin_bit_cast(T, b));
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < RUN; k++) v[k] = k < n ? to_f(p[k]) : 0.0f;
+}
+
+template <typename T, int RUN>
+__device__ __forceinline__ void store_run(T* p, const float (&v)[RUN], int64_t n) {
+  if (n >= RUN) {
+    u32x4 w;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < RUN; k++) w[k] = __float_as_uint(v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < RUN; k += 2)
+        w[k >> 1] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<T>(v[k])) |
+                    (uint32_t)__builtin_bit_cast(uint16_t, from_f<T>(v[k + 1])) << 16;
+    }
+    ((Bytes16*)p)->v = w;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < RUN; k++)
+    if (k < n) p[k] = from_f<T>(v[k]);
+}
+
+// One result in plain 32-bit arithmetic, r in [r0, r1) of each segment.
+__device__ __noinline__ float exact_sum(const float* a, int64_t a_i, int64_t a_r, const float* b0,
+                                        const float* b1, int64_t b_j, int64_t b_r, int segments,
+                                        int64_t a_segment, int64_t i, int64_t j, int64_t r0, int64_t r1) {
+  float v = 0.0f;
+  for (int s = 0; s < segments; s++) {
+    const float* A = a + s * a_segment + i * a_i;
+    const float* B = (s ? b1 : b0) + j * b_j;
+    for (int64_t r = r0; r < r1; r++) v = fmaf(A[r * a_r], b0 ? B[r * b_r] : 1.0f, v);
+  }
+  return v;
+}
+
+// The tiles of C, j fastest, then i, then the ranges of r: consecutive tiles share rows of A.
+// Workgroups go to the 8 XCDs in turn, so XCD x takes the x-th eighth of them: tiles that share
+// operands share an L2.
+struct Place {
+  int64_t i;  // tile
+  uint32_t j, split;
+  bool in;
+};
+__device__ __forceinline__ Place place(uint32_t tiles_i, uint32_t tiles_j, uint32_t splits) {
+  const uint32_t total = tiles_i * tiles_j * splits, each = gridDim.x >> 3;
+  const uint32_t t = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  Place p;
+  p.in = t < total;
+  p.j = t % tiles_j;
+  const uint32_t rest = t / tiles_j;
+  p.i = rest % tiles_i;
+  p.split = rest / tiles_i;
+  return p;
+}
+
+// WI x WJ waves; a wave has BI / WI rows i and BJ / WJ rows j of the tile.  GATED: the tile's BJ
+// rows are BJ / 2 of the gate's weights and the same BJ / 2 of the up weights.
+template <typename T, bool RCA, bool RCB, int EPI, bool GATED, int BI, int WI, int BJ, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, uint32_t tiles_i,
+                                                               uint32_t tiles_j, uint32_t splits) {
+  constexpr int NT = 64 * WI * WJ, kDepth = Operand<T>::kDepth, kPlanes = Operand<T>::kPlanes;
+  constexpr int kBuffers = Operand<T>::kBuffers;
+  constexpr int NI = BI / WI / 16, NJ = BJ / WJ / 16;  // 16x16 tiles of a wave
+  constexpr bool kPaired = sizeof(T) == 2 && EPI != EPI_PARTIAL;
+  constexpr int RUN = kPaired ? 8 : 4;
+  constexpr int kOut = GATED ? BJ / 2 : BJ;  // outputs of the tile
+  static_assert(!GATED || (WJ == 1 && RCB), "");
+  using TA = Tile<T, RCA, BI, NT, false>;
+  using TB = Tile<T, RCB, BJ, NT, kPaired>;
+  __shared__ __attribute__((aligned(256))) char lds[kBuffers * (TA::kBytes + TB::kBytes)];
+
+  const Place at = place(tiles_i, tiles_j, splits);
+  if (!at.in) return;
+  const int wave = threadIdx.x >> 6, wi = wave / WJ, wj = wave % WJ;
+  const int64_t i0 = at.i * BI, j0 = (int64_t)at.j * kOut;
+  int64_t r_begin = 0, r_end = p.R;
+  if (EPI == EPI_PARTIAL) {
+    r_begin = (int64_t)at.split * p.r_chunk;
+    r_end = r_begin + p.r_chunk < p.R ? r_begin + p.r_chunk : p.R;
+  }
+  const int64_t lda = RCA ? p.a_i : p.a_r, ldb = RCB ? p.b_j : p.b_r;
+  const uint32_t steps = (uint32_t)((r_end - r_begin + kDepth - 1) / kDepth);
+  const uint32_t total = EPI == EPI_PLAIN ? steps * p.segments : steps;
+  const bool inside = i0 + BI <= p.I && j0 + kOut <= p.J;
+
+  Chunk<T> ca[TA::kChunks], cb[TB::kChunks];
+  auto load = [&](uint32_t it) {
+    const T* a = (const T*)p.a;
+    const T* b = (const T*)p.b[0];
+    if (EPI == EPI_PLAIN && it >= steps) {  // the second segment
+      it -= steps;
+      a += p.a_segment;
+      b = (const T*)p.b[1];
+    }
+    const int64_t r0 = r_begin + (int64_t)it * kDepth;
+    constexpr int kSplit = GATED ? BJ / 2 : 0;
+    if (inside && r0 + kDepth <= r_end) {
+      TA::template load<true, 0>(ca, a, nullptr, lda, i0, p.I, r0, r_end);
+      TB::template load<true, kSplit>(cb, b, (const T*)p.b[1], ldb, j0, p.J, r0, r_end);
+    } else {
+      TA::template load<false, 0>(ca, a, nullptr, lda, i0, p.I, r0, r_end);
+      TB::template load<false, kSplit>(cb, b, (const T*)p.b[1], ldb, j0, p.J, r0, r_end);
+    }
+  };
+  auto store = [&](int buffer) {
+    char* s = lds + buffer * (TA::kBytes + TB::kBytes);
+    TA::store(s, ca);
+    TB::store(s + TA::kBytes, cb);
+  };
+
+  f32x4 acc[NI][NJ] = {}, sum[NI] = {};
+  const bool sums = EPI == EPI_PARTIAL && p.part_sum && at.j == 0 && wj == 0;
+  auto compute = [&](int buffer) {
+    const char* sa = lds + buffer * (TA::kBytes + TB::kBytes);
+    const char* sb = sa + TA::kBytes;
+#pragma unroll
+    for (int kk = 0; kk < kDepth / 32; kk++) {
+      s16x8 b[NJ][kPlanes];
+#pragma unroll
+      for (int t = 0; t < NJ; t++)
+#pragma unroll
+        for (int q = 0; q < kPlanes; q++) b[t][q] = TB::read(sb + q * TB::kPlaneBytes, wj * NJ + t, kk);
+#pragma unroll
+      for (int u = 0; u < NI; u++) {
+        s16x8 a[kPlanes];
+#pragma unroll
+        for (int q = 0; q < kPlanes; q++) a[q] = TA::read(sa + q * TA::kPlaneBytes, wi * NI + u, kk);
+        if constexpr (kPlanes == 1) {
+#pragma unroll
+          for (int t = 0; t < NJ; t++) acc[u][t] = mfma<T>(b[t][0], a[0], acc[u][t]);
+        } else {
+          // smallest products first; consecutive instructions work on different results
+          constexpr int kA[6] = {2, 0, 1, 1, 0, 0}, kB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+          for (int k = 0; k < 6; k++)
+#pragma unroll
+            for (int t = 0; t < NJ; t++) acc[u][t] = mfma<T>(b[t][kB[k]], a[kA[k]], acc[u][t]);
+        }
+        if (EPI == EPI_PARTIAL && sums) {  // the bias gradient: the same rows times ones
+          const short one = sizeof(T) == 2 && __is_same(T, __half) ? 0x3c00 : 0x3f80;
+          const s16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+          for (int q = kPlanes - 1; q >= 0; q--) sum[u] = mfma<T>(ones, a[q], sum[u]);
+        }
+      }
+    }
+  };
+
+  load(0);
+  if constexpr (kBuffers == 2) {
+    store(0);
+    for (uint32_t it = 0; it < total; it++) {
+      __syncthreads();  // everyone has stored this step and left the other buffer
+      if (it + 1 < total) load(it + 1);
+      compute(it & 1);
+      if (it + 1 < total) store((it + 1) & 1);
+    }
+  } else {
+    for (uint32_t it = 0; it < total; it++) {
+      if (it) __syncthreads();  // everyone has left the buffer
+      store(0);
+      __syncthreads();
+      if (it + 1 < total) load(it + 1);
+      compute(0);
+    }
+  }
+
+  const int m = threadIdx.x & 15, q = (threadIdx.x & 63) >> 4;
+  if constexpr (sizeof(T) == 4) {
+    float odd = 0.0f;  // stays 0 while every result is finite
+#pragma unroll
+    for (int u = 0; u < NI; u++) {
+#pragma unroll
+      for (int t = 0; t < NJ; t++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) odd = fmaf(acc[u][t][v], 0.0f, odd);
+      if (sums) odd = fmaf(sum[u][0], 0.0f, odd);
+    }
+    if (odd != 0.0f) {
+#pragma unroll
+      for (int u = 0; u < NI; u++) {
+        const int64_t i = i0 + (wi * NI + u) * 16 + m;
+        if (i >= p.I) continue;
+        const int segments = EPI == EPI_PLAIN ? p.segments : 1;
+#pragma unroll
+        for (int t = 0; t < NJ; t++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) {
+            const int row = (wj * NJ + t) * 16 + 4 * q + v;
+            const bool second = GATED && row >= kOut;
+            const int64_t j = j0 + (second ? row - kOut : row);
+            if (j < p.J && !(fabsf(acc[u][t][v]) <= 3.4e38f))
+              acc[u][t][v] = exact_sum((const float*)p.a, p.a_i, p.a_r, (const float*)p.b[second ? 1 : 0],
+                                       (const float*)p.b[1], p.b_j, p.b_r, segments, p.a_segment, i, j,
+                                       r_begin, r_end);
+          }
+        if (sums && !(fabsf(sum[u][0]) <= 3.4e38f))
+          sum[u][0] = exact_sum((const float*)p.a, p.a_i, p.a_r, nullptr, nullptr, 0, 0, 1, 0, i, 0, r_begin, r_end);
+      }
+    }
+  }
+
+  if (EPI == EPI_PARTIAL && sums && q == 0) {
+#pragma unroll
+    for (int u = 0; u < NI; u++) {
+      const int64_t i = i0 + (wi * NI + u) * 16 + m;
+      if (i < p.I) p.part_sum[(int64_t)at.split * p.I + i] = sum[u][0];
+    }
+  }
+  constexpr int kRuns = NJ * 4 / RUN / (GATED ? 2 : 1);
+#pragma unroll
+  for (int s = 0; s < kRuns; s++) {
+    const int64_t j = j0 + wj * (NJ * 16) + (kPaired ? 32 * s + 8 * q : 16 * s + 4 * q);
+    const int64_t n = p.J - j;
+    if (n <= 0) continue;
+    float bias[RUN] = {}, bias1[RUN] = {};
+    if (EPI == EPI_FORWARD || EPI == EPI_DZ) {
+      if (p.bias[0]) load_run<T, RUN>(bias, (const T*)p.bias[0] + j, n);
+      if (GATED && p.bias[1]) load_run<T, RUN>(bias1, (const T*)p.bias[1] + j, n);
+    }
+#pragma unroll
+    for (int u = 0; u < NI; u++) {
+      const int64_t i = i0 + (wi * NI + u) * 16 + m;
+      if (i >= p.I) continue;
+      float v[RUN], w[RUN], ex[RUN] = {};
+#pragma unroll
+      for (int k = 0; k < RUN; k++) {
+        v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4] + bias[k];
+        if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4] + bias1[k];
+      }
+      if (EPI == EPI_PARTIAL) {
+        store_run<float, 4>(p.part + ((int64_t)at.split * p.I + i) * p.J + j, (const float(&)[4])v, n);
+        continue;
+      }
+      if ((EPI == EPI_FORWARD || EPI == EPI_DZ) && p.extra)
+        load_run<T, RUN>(ex, (const T*)p.extra + i * p.extra_row + j, n);
+      T* out = (T*)p.out + i * p.out_row + j;
+      if (EPI == EPI_FORWARD) {
+#pragma unroll
+        for (int k = 0; k < RUN; k++) v[k] = GATED ? act_value(v[k], p.act) * w[k] : act_value(v[k], p.act) + ex[k];
+      } else if (EPI == EPI_DZ) {
+#pragma unroll
+        for (int k = 0; k < RUN; k++) {
+          if (GATED) {
+            const float d = ex[k] * act_value(v[k], p.act);
+            v[k] = ex[k] * w[k] * act_slope(v[k], p.act);
+            w[k] = d;
+          } else {
+            v[k] = ex[k] * act_slope(v[k], p.act);
+          }
+        }
+        if (GATED) store_run<T, RUN>(out + p.J, w, n);
+      }
+      store_run<T, RUN>(out, v, n);
+    }
+  }
+}
+
+template <typename T, bool RCA, bool RCB, int EPI, bool GATED, int BI, int WI, int BJ, int WJ>
+int launch_product(const ProductArgs& p, int64_t splits, hipStream_t stream) {
+  constexpr int kOut = GATED ? BJ / 2 : BJ;
+  const int64_t ti = (p.I + BI - 1) / BI, tj = (p.J + kOut - 1) / kOut;
+  if (ti > 0x7fffffff / tj || ti * tj > 0x7ffffff0 / splits) return 1;
+  const int64_t total = ti * tj * splits, grid = (total + 7) / 8 * 8;
+  hipLaunchKernelGGL((product_kernel<T, RCA, RCB, EPI, GATED, BI, WI, BJ, WJ>), dim3((uint32_t)grid),
+                     dim3(64 * WI * WJ), 0, stream, p, (uint32_t)ti, (uint32_t)tj, (uint32_t)splits);
+  return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+
+// The tile by the size of C: 128 x 128 where there are outputs for it, 128 x 64 for narrow
+// results, 64 x 64 where the larger ones would leave CUs without work.
+template <typename T, bool RCA, bool RCB, int EPI>
+int launch_linear(const ProductArgs& p, int64_t splits, hipStream_t stream) {
+  const int64_t large = (p.I + 127) / 128 * ((p.J + 127) / 128) * splits;
+  if (p.J > 64 && large >= 256) return launch_product<T, RCA, RCB, EPI, false, 128, 2, 128, 2>(p, splits, stream);
+  if (p.J <= 64 && (p.I + 127) / 128 * splits >= 256)
+    return launch_product<T, RCA, RCB, EPI, false, 128, 4, 64, 1>(p, splits, stream);
+  return launch_product<T, RCA, RCB, EPI, false, 64, 4, 64, 1>(p, splits, stream);
+}
+
+template <typename T, int EPI>
+int launch_gated(const ProductArgs& p, hipStream_t stream) {
+  const int64_t large = (p.I + 127) / 128 * ((p.J + 63) / 64);
+  if (large >= 256) return launch_product<T, true, true, EPI, true, 128, 4, 128, 1>(p, 1, stream);
+  return launch_product<T, true, true, EPI, true, 64, 4, 128, 1>(p, 1, stream);
+}
+
+// What gsr_linear.hip needs of each type (gsr_linear_f32.hip, _f16.hip, _bf16.hip).
+template <typename T> int product_forward(const ProductArgs& p, bool gated, hipStream_t s);
+template <typename T> int product_dz(const ProductArgs& p, bool gated, hipStream_t s);
+template <typename T> int product_dx(const ProductArgs& p, hipStream_t s);
+template <typename T> int product_dw(const ProductArgs& p, int64_t splits, hipStream_t s);
+
+#define GSR_PRODUCTS(T)                                                                              \
+  template <> int product_forward<T>(const ProductArgs& p, bool gated, hipStream_t s) {              \
+    if (gated) return launch_gated<T, EPI_FORWARD>(p, s);                                            \
+    return p.a_r == 1 ? launch_linear<T, true, true, EPI_FORWARD>(p, 1, s)                           \
+                      : launch_linear<T, false, true, EPI_FORWARD>(p, 1, s);                         \
+  }                                                                                                  \
+  template <> int product_dz<T>(const ProductArgs& p, bool gated, hipStream_t s) {                   \
+    if (gated) return launch_gated<T, EPI_DZ>(p, s);                                                 \
+    return p.a_r == 1 ? launch_linear<T, true, true, EPI_DZ>(p, 1, s)                                \
+                      : launch_linear<T, false, true, EPI_DZ>(p, 1, s);                              \
+  }                                                                                                  \
+  template <> int product_dx<T>(const ProductArgs& p, hipStream_t s) {                               \
+    return launch_linear<T, true, false, EPI_PLAIN>(p, 1, s);                                        \
+  }                                                                                                  \
+  template <> int product_dw<T>(const ProductArgs& p, int64_t splits, hipStream_t s) {               \
+    return p.b_j == 1 ? launch_linear<T, false, false, EPI_PARTIAL>(p, splits, s)                    \
+                      : launch_linear<T, false, true, EPI_PARTIAL>(p, splits, s);                    \
+  }
+
+}  // namespace gsr
