@@ -30,10 +30,11 @@ enum { GSR_F32 = 0, GSR_F16 = 1, GSR_BF16 = 2 };
 enum { GSR_ACT_NONE = 0, GSR_ACT_RELU = 1, GSR_ACT_GELU = 2, GSR_ACT_SILU = 3 };
 
 /* y = act(x w^T + bias) + residual.  bias, residual may be NULL.  gelu is the erf form. */
+size_t gsr_linear_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N);
 int gsr_linear(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,
                int64_t x_col, const void* w, int64_t w_row, const void* bias,
                const void* residual, int64_t residual_row, int act, void* y, int64_t y_row,
-               void* stream);
+               void* scratch, void* stream);
 
 /* Gradients of gsr_linear: with z = x w^T + bias (computed again, so a forward keeps nothing)
  * and dz = dy act'(z): dx = dz w [M,K], dw = dz^T x [N,K], dbias = the column sums of dz [N], all
@@ -47,9 +48,10 @@ int gsr_linear_backward(int dtype, int64_t M, int64_t K, int64_t N, const void* 
 
 /* h = act(x wg^T + bg) * (x wu^T + bu), both products in one pass over x [M,K] (rows contiguous).
  * bg and bu may be NULL. */
+size_t gsr_gated_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N);
 int gsr_gated(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,
               const void* wg, const void* wu, int64_t w_row, const void* bg, const void* bu,
-              int act, void* h, int64_t h_row, void* stream);
+              int act, void* h, int64_t h_row, void* scratch, void* stream);
 
 /* Gradients of gsr_gated (g, u computed again): dg = dh u act'(g), du = dh act(g);
  * dx = dg wg + du wu [M,K]; dw [2N,K] = the gradients of wg and then wu; db [2N] likewise.  Any of

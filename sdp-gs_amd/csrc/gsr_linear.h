@@ -62,27 +62,33 @@ __device__ __forceinline__ float normal_cdf(float z, float& e) {
   return z < 0.0f ? tail : 1.0f - tail;
 }
 
-__device__ __forceinline__ float act_value(float z, int act) {
-  if (act == GSR_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-  if (act == GSR_ACT_GELU) {
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == GSR_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
+  if constexpr (ACT == GSR_ACT_GELU) {
     float e;
     return z * normal_cdf(z, e);
   }
-  if (act == GSR_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+  if constexpr (ACT == GSR_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
   return z;
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == GSR_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (act == GSR_ACT_GELU) {
+// The activation's value and slope at z.
+template <int ACT>
+__device__ __forceinline__ float act_both(float z, float& value) {
+  if constexpr (ACT == GSR_ACT_GELU) {
     float e;
     const float c = normal_cdf(z, e);
+    value = z * c;
     return fmaf(z * 0.39894228040143268f, e, c);
   }
-  if (act == GSR_ACT_SILU) {
+  if constexpr (ACT == GSR_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+    value = z * s;
     return s * fmaf(z, 1.0f - s, 1.0f);
   }
+  value = act_value<ACT>(z);
+  if constexpr (ACT == GSR_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   return 1.0f;
 }
 

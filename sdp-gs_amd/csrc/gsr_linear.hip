@@ -27,7 +27,6 @@ __global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
   if (e < n) p[e] = from_f<T>(0.0f);
 }
 
-size_t type_bytes(int dtype) { return dtype == GSR_F32 ? 4 : 2; }
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // Ranges of the summed rows for dw: enough 128 x 128 tiles to fill 256 CUs twice, each with at
@@ -81,6 +80,21 @@ size_t partial_bytes(int64_t M, int64_t K, int64_t I) {
   return M == 0 ? 0 : (size_t)ranges_of(I, K, M).count * I * (K + 1) * 4;
 }
 
+// Scratch of a backward, in order: the pre-activation gradients, then what one product at a time
+// needs (the weights' images, the partial sums).
+template <typename T>
+size_t backward_bytes(int64_t M, int64_t K, int64_t N, bool gated, bool has_dz, bool need_dw) {
+  const int64_t width = gated ? 2 * N : N;
+  size_t most = has_dz ? product_scratch<T>(M, N, K, gated) : 0;
+  if (!gated) {
+    const size_t dx = product_scratch<T>(M, K, N, false);
+    most = dx > most ? dx : most;
+  }
+  const size_t dw = need_dw ? partial_bytes(M, K, width) : 0;
+  most = dw > most ? dw : most;
+  return (has_dz ? (size_t)up(M * width * sizeof(T), 256) : 0) + most;
+}
+
 template <typename T>
 int linear_backward(const ProductArgs& fwd, const void* dy, int64_t dy_row, void* dx, void* dw,
                     void* db, char* scratch, hipStream_t stream) {
@@ -91,9 +105,9 @@ int linear_backward(const ProductArgs& fwd, const void* dy, int64_t dy_row, void
     ProductArgs p = fwd;
     p.extra = dy; p.extra_row = dy_row;
     p.out = scratch; p.out_row = N;
-    if (int rc = product_dz<T>(p, false, stream)) return rc;
     dz = scratch; dz_row = N;
     scratch += up(M * N * sizeof(T), 256);
+    if (int rc = product_dz<T>(p, false, scratch, stream)) return rc;
   }
   if (dx && M > 0) {
     ProductArgs p{};
@@ -101,7 +115,7 @@ int linear_backward(const ProductArgs& fwd, const void* dy, int64_t dy_row, void
     p.b[0] = fwd.b[0]; p.b_j = 1; p.b_r = fwd.b_j;
     p.I = M; p.J = K; p.R = N; p.segments = 1;
     p.out = dx; p.out_row = K;
-    if (int rc = product_dx<T>(p, stream)) return rc;
+    if (int rc = product_dx<T>(p, scratch, stream)) return rc;
   }
   if (!dw && !db) return 0;
   return weight_gradients<T>(dz, dz_row, M, K, N, fwd.a, fwd.a_i, fwd.a_r, dw, db, scratch, stream);
@@ -116,15 +130,15 @@ int gated_backward(const ProductArgs& fwd, const void* dh, int64_t dh_row, void*
     ProductArgs p = fwd;
     p.extra = dh; p.extra_row = dh_row;
     p.out = scratch; p.out_row = 2 * N;
-    if (int rc = product_dz<T>(p, true, stream)) return rc;
     scratch += up(2 * M * N * sizeof(T), 256);
+    if (int rc = product_dz<T>(p, true, scratch, stream)) return rc;
     if (dx) {
       ProductArgs q{};
       q.a = dz; q.a_i = 2 * N; q.a_r = 1;
       q.b[0] = fwd.b[0]; q.b[1] = fwd.b[1]; q.b_j = 1; q.b_r = fwd.b_j;
       q.I = M; q.J = K; q.R = N; q.segments = 2; q.a_segment = N;
       q.out = dx; q.out_row = K;
-      if (int rc = product_dx<T>(q, stream)) return rc;
+      if (int rc = product_dx<T>(q, scratch, stream)) return rc;
     }
   }
   if (!dw && !db) return 0;
@@ -143,32 +157,53 @@ ProductArgs forward_args(int64_t M, int64_t K, int64_t N, const void* x, int64_t
   return p;
 }
 
-int forward(int dtype, const ProductArgs& p, bool gated, hipStream_t s) {
-  if (dtype == GSR_F32) return product_forward<float>(p, gated, s);
-  if (dtype == GSR_F16) return product_forward<__half>(p, gated, s);
-  return product_forward<__hip_bfloat16>(p, gated, s);
+// f(a null pointer of the call's type)
+template <typename F>
+auto with_type(int dtype, F f) {
+  if (dtype == GSR_F32) return f((float*)nullptr);
+  if (dtype == GSR_F16) return f((__half*)nullptr);
+  return f((__hip_bfloat16*)nullptr);
+}
+template <typename P> struct Pointee;
+template <typename T> struct Pointee<T*> { using type = T; };
+
+int forward(int dtype, const ProductArgs& p, bool gated, void* scratch, void* stream) {
+  return with_type(dtype, [&](auto t) {
+    return product_forward<typename Pointee<decltype(t)>::type>(p, gated, (char*)scratch, (hipStream_t)stream);
+  });
+}
+
+size_t forward_bytes(int dtype, int64_t M, int64_t K, int64_t N, bool gated) {
+  return with_type(dtype, [&](auto t) {
+    return product_scratch<typename Pointee<decltype(t)>::type>(M, N, K, gated);
+  }) + 256;
 }
 
 }  // namespace
 
+extern "C" size_t gsr_linear_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
+  return sizes_ok(dtype, M, K, N, GSR_ACT_NONE) ? forward_bytes(dtype, M, K, N, false) : 0;
+}
+
 extern "C" int gsr_linear(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,
                           int64_t x_col, const void* w, int64_t w_row, const void* bias,
                           const void* residual, int64_t residual_row, int act, void* y,
-                          int64_t y_row, void* stream) {
+                          int64_t y_row, void* scratch, void* stream) {
   if (!sizes_ok(dtype, M, K, N, act) || !x_ok(M, K, x_row, x_col) || w_row < K) return 1;
   if (M == 0) return 0;
-  if (!x || !w || !y || y_row < N || (residual && residual_row < N && M > 1)) return 1;
+  if (!x || !w || !y || !scratch || y_row < N || (residual && residual_row < N && M > 1)) return 1;
   ProductArgs p = forward_args(M, K, N, x, x_row, x_col, w, nullptr, w_row, bias, nullptr, act);
   p.extra = residual; p.extra_row = residual_row;
   p.out = y; p.out_row = y_row;
-  return forward(dtype, p, false, (hipStream_t)stream);
+  return forward(dtype, p, false, scratch, stream);
 }
 
 extern "C" size_t gsr_linear_backward_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N,
                                                     int act, int need_dw) {
   if (!sizes_ok(dtype, M, K, N, act)) return 0;
-  return (act == GSR_ACT_NONE ? 0 : (size_t)up(M * N * type_bytes(dtype), 256)) +
-         (need_dw ? partial_bytes(M, K, N) : 0) + 256;
+  return with_type(dtype, [&](auto t) {
+    return backward_bytes<typename Pointee<decltype(t)>::type>(M, K, N, false, act != GSR_ACT_NONE, need_dw);
+  }) + 256;
 }
 
 extern "C" int gsr_linear_backward(int dtype, int64_t M, int64_t K, int64_t N, const void* x,
@@ -180,27 +215,32 @@ extern "C" int gsr_linear_backward(int dtype, int64_t M, int64_t K, int64_t N, c
   const ProductArgs p = forward_args(M, K, N, x, x_row, x_col, w, nullptr, w_row, bias, nullptr, act);
   hipStream_t s = (hipStream_t)stream;
   char* t = (char*)scratch;
-  if (dtype == GSR_F32) return linear_backward<float>(p, dy, dy_row, dx, dw, dbias, t, s);
-  if (dtype == GSR_F16) return linear_backward<__half>(p, dy, dy_row, dx, dw, dbias, t, s);
-  return linear_backward<__hip_bfloat16>(p, dy, dy_row, dx, dw, dbias, t, s);
+  return with_type(dtype, [&](auto k) {
+    return linear_backward<typename Pointee<decltype(k)>::type>(p, dy, dy_row, dx, dw, dbias, t, s);
+  });
+}
+
+extern "C" size_t gsr_gated_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
+  return sizes_ok(dtype, M, K, N, GSR_ACT_NONE) ? forward_bytes(dtype, M, K, N, true) : 0;
 }
 
 extern "C" int gsr_gated(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,
                          const void* wg, const void* wu, int64_t w_row, const void* bg,
-                         const void* bu, int act, void* h, int64_t h_row, void* stream) {
+                         const void* bu, int act, void* h, int64_t h_row, void* scratch, void* stream) {
   if (!sizes_ok(dtype, M, K, N, act) || !x_ok(M, K, x_row, 1) || w_row < K) return 1;
   if (M == 0) return 0;
-  if (!x || !wg || !wu || !h || h_row < N) return 1;
+  if (!x || !wg || !wu || !h || !scratch || h_row < N) return 1;
   ProductArgs p = forward_args(M, K, N, x, x_row, 1, wg, wu, w_row, bg, bu, act);
   p.out = h; p.out_row = h_row;
-  return forward(dtype, p, true, (hipStream_t)stream);
+  return forward(dtype, p, true, scratch, stream);
 }
 
 extern "C" size_t gsr_gated_backward_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N,
                                                    int need_dw) {
   if (!sizes_ok(dtype, M, K, N, GSR_ACT_NONE)) return 0;
-  return (size_t)up(2 * M * N * type_bytes(dtype), 256) + (need_dw ? partial_bytes(M, K, 2 * N) : 0) +
-         256;
+  return with_type(dtype, [&](auto t) {
+    return backward_bytes<typename Pointee<decltype(t)>::type>(M, K, N, true, true, need_dw);
+  }) + 256;
 }
 
 extern "C" int gsr_gated_backward(int dtype, int64_t M, int64_t K, int64_t N, const void* x,
@@ -213,7 +253,7 @@ extern "C" int gsr_gated_backward(int dtype, int64_t M, int64_t K, int64_t N, co
   const ProductArgs p = forward_args(M, K, N, x, x_row, 1, wg, wu, w_row, bg, bu, act);
   hipStream_t s = (hipStream_t)stream;
   char* t = (char*)scratch;
-  if (dtype == GSR_F32) return gated_backward<float>(p, dh, dh_row, dx, dw, db, t, s);
-  if (dtype == GSR_F16) return gated_backward<__half>(p, dh, dh_row, dx, dw, db, t, s);
-  return gated_backward<__hip_bfloat16>(p, dh, dh_row, dx, dw, db, t, s);
+  return with_type(dtype, [&](auto k) {
+    return gated_backward<typename Pointee<decltype(k)>::type>(p, dh, dh_row, dx, dw, db, t, s);
+  });
 }

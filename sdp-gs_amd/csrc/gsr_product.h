@@ -61,28 +61,88 @@ template <typename T> struct Chunk {
   u32x4 w[Operand<T>::kRaw];
 };
 
-// n of the 8 elements at p exist (n <= 0: none); the others are zero.
-template <typename T, bool FULL>
-__device__ __forceinline__ Chunk<T> load_chunk(const T* p, int64_t n) {
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_whole(const T* p) {
   Chunk<T> c;
-  if (FULL || n >= 8) {
 #pragma unroll
-    for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = ((const Bytes16*)p)[k].v;
-    return c;
-  }
+  for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = ((const Bytes16*)p)[k].v;
+  return c;
+}
+
+// Elements k..k+7 of a row of n (n >= 1) that are `step` apart; those past its end are zero.  Every
+// load is made, from the last element where there is none: no branch, so all are in flight at once.
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_tail(const T* row, int64_t k, int64_t step, int64_t n) {
+  Chunk<T> c;
 #pragma unroll
-  for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = u32x4{0, 0, 0, 0};
-  if (n <= 0) return c;
-  if constexpr (sizeof(T) == 4) {
+  for (int e = 0; e < Operand<T>::kRaw; e++) c.w[e] = u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 7; e++)
-      if (e < n) c.w[e >> 2][e & 3] = ((const uint32_t*)p)[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 7; e++)
-      if (e < n) c.w[0][e >> 1] |= (uint32_t)((const uint16_t*)p)[e] << (16 * (e & 1));
+  for (int e = 0; e < 8; e++) {
+    const int64_t at = (k + e < n ? k + e : n - 1) * step;
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t v = ((const uint32_t*)row)[at];
+      c.w[e >> 2][e & 3] = k + e < n ? v : 0u;
+    } else {
+      const uint32_t v = ((const uint16_t*)row)[at];
+      c.w[0][e >> 1] |= (k + e < n ? v : 0u) << (16 * (e & 1));
+    }
   }
   return c;
+}
+// 16 bytes of a row of n elements from element k on; those past its end repeat its last.
+template <typename T>
+__device__ __forceinline__ u32x4 load_tail_words(const T* row, int64_t k, int64_t n) {
+  u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < (int)(16 / sizeof(T)); e++) {
+    const int64_t at = k + e < n ? k + e : n - 1;
+    if constexpr (sizeof(T) == 4) w[e] = ((const uint32_t*)row)[at];
+    else w[e >> 1] |= (uint32_t)((const uint16_t*)row)[at] << (16 * (e & 1));
+  }
+  return w;
+}
+
+// Which parts are multiplied: smallest products first.
+template <int PLANES> struct Parts {
+  static constexpr int kProducts = 1, kA[1] = {0}, kB[1] = {0};
+};
+template <> struct Parts<3> {
+  static constexpr int kProducts = 6, kA[6] = {2, 0, 1, 1, 0, 0}, kB[6] = {0, 2, 1, 0, 1, 0};
+};
+
+// Waits for this wave's LDS accesses, then for the other waves; global accesses stay in flight.
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// The 8 elements as 16-bit parts.
+template <typename T>
+__device__ __forceinline__ void split_chunk(s16x8 (&part)[Operand<T>::kPlanes], const Chunk<T>& c) {
+  if constexpr (Operand<T>::kPlanes == 1) {
+    part[0] = __builtin_bit_cast(s16x8, c.w[0]);
+  } else {
+    u32x4 w[3];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      f32x2 v = {__uint_as_float(c.w[k >> 1][(k & 1) * 2]), __uint_as_float(c.w[k >> 1][(k & 1) * 2 + 1])};
+#pragma unroll
+      for (int p = 0; p < 3; p++) {
+        w[p][k] = round_pair(v);
+        v -= widen_pair(w[p][k]);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 3; p++) part[p] = __builtin_bit_cast(s16x8, w[p]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put_chunk(char* to, int plane_bytes, const Chunk<T>& c) {
+  s16x8 part[Operand<T>::kPlanes];
+  split_chunk<T>(part, c);
+#pragma unroll
+  for (int p = 0; p < Operand<T>::kPlanes; p++) *(s16x8*)(to + p * plane_bytes) = part[p];
 }
 
 // One operand's tile in LDS.  RC: contiguous along r (rows of kDepth), else rows of ROWS.
@@ -107,23 +167,28 @@ struct Tile {
     return PAIRED ? ((row >> 1) & 1) | (((row >> 3) & 3) << 1) : (row >> 1) & 7;
   }
 
-  // Rows [o0, o0 + ROWS) of O, r in [r0, r0 + kDepth) below r_end.  base1: rows from SPLIT on.
-  template <bool FULL, int SPLIT>
+  // Rows [o0, o0 + ROWS) of O, r in [r0, r0 + kDepth) below r_end (zeros from there on).  A row past
+  // the last is some other row: its results are not stored.  base1: rows from SPLIT on.
+  template <int SPLIT>
   static __device__ __forceinline__ void load(Chunk<T> (&c)[kChunks], const T* base, const T* base1,
                                               int64_t ld, int64_t o0, int64_t O, int64_t r0, int64_t r_end) {
+    const bool whole = r0 + kDepth <= r_end && (RC || o0 + ROWS <= O);
 #pragma unroll
     for (int s = 0; s < kChunks; s++) {
       const int q = s * THREADS + threadIdx.x, row = q / kPerRow, col = q % kPerRow * 8;
       if (RC) {
         const bool second = SPLIT && row >= SPLIT;
-        const int64_t o = o0 + (second ? row - SPLIT : row);
-        const T* b = second ? base1 : base;
-        if (FULL) c[s] = load_chunk<T, true>(b + o * ld + r0 + col, 8);
-        else c[s] = load_chunk<T, false>(b + o * ld + r0 + col, o < O ? r_end - r0 - col : 0);
+        int64_t o = o0 + (second ? row - SPLIT : row);
+        o = o < O ? o : O - 1;
+        const T* p = (second ? base1 : base) + o * ld;
+        c[s] = whole ? load_whole(p + r0 + col) : load_tail(p, r0 + col, 1, r_end);
+      } else if (whole) {
+        c[s] = load_whole(base + (r0 + row) * ld + o0 + col);
       } else {
-        const T* p = base + (r0 + row) * ld + o0 + col;
-        if (FULL) c[s] = load_chunk<T, true>(p, 8);
-        else c[s] = load_chunk<T, false>(p, r0 + row < r_end ? O - o0 - col : 0);
+        const bool in = r0 + row < r_end;
+        c[s] = load_tail(base + (in ? r0 + row : r_end - 1) * ld, o0 + col, 1, O);
+#pragma unroll
+        for (int k = 0; k < Operand<T>::kRaw; k++) c[s].w[k] = in ? c[s].w[k] : u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -132,23 +197,7 @@ struct Tile {
 #pragma unroll
     for (int s = 0; s < kChunks; s++) {
       const int q = s * THREADS + threadIdx.x, row = q / kPerRow, at = q % kPerRow ^ swizzle(row);
-      u32x4* to = (u32x4*)(lds + (row * kPerRow + at) * 16);
-      if constexpr (kPlanes == 1) {
-        *to = c[s].w[0];
-      } else {
-        u32x4 part[3];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          f32x2 v = {__uint_as_float(c[s].w[k >> 1][(k & 1) * 2]), __uint_as_float(c[s].w[k >> 1][(k & 1) * 2 + 1])};
-#pragma unroll
-          for (int p = 0; p < 3; p++) {
-            part[p][k] = round_pair(v);
-            v -= widen_pair(part[p][k]);
-          }
-        }
-#pragma unroll
-        for (int p = 0; p < 3; p++) *(u32x4*)((char*)to + p * kPlaneBytes) = part[p];
-      }
+      put_chunk<T>(lds + (row * kPerRow + at) * 16, kPlaneBytes, c[s]);
     }
   }
 
@@ -171,25 +220,42 @@ struct Tile {
   }
 };
 
-// RUN consecutive elements of a row as floats; `n` of them exist.
+// 16 bytes of a row, RUN elements, as floats and back; `n` of them exist.
+template <typename T>
+__device__ __forceinline__ u32x4 load_words(const T* p, int64_t n) {
+  constexpr int RUN = 16 / sizeof(T);
+  if (n >= RUN) return ((const Bytes16*)p)->v;
+  u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < RUN - 1; k++) {
+    if (k >= n) break;
+    if constexpr (sizeof(T) == 4) w[k] = ((const uint32_t*)p)[k];
+    else w[k >> 1] |= (uint32_t)((const uint16_t*)p)[k] << (16 * (k & 1));
+  }
+  return w;
+}
+template <typename T, int RUN>
+__device__ __forceinline__ void widen(float (&v)[RUN], u32x4 w) {
+#pragma unroll
+  for (int k = 0; k < RUN; k++) {
+    if constexpr (sizeof(T) == 4) v[k] = __uint_as_float(w[k]);
+    else if constexpr (__is_same(T, __half)) v[k] = to_f(__builtin_bit_cast(__half, (uint16_t)(w[k >> 1] >> (16 * (k & 1)))));
+    else v[k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+  }
+}
 template <typename T, int RUN>
 __device__ __forceinline__ void load_run(float (&v)[RUN], const T* p, int64_t n) {
-  if (n >= RUN) {
-    const u32x4 w = ((const Bytes16*)p)->v;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int k = 0; k < RUN; k++) v[k] = __uint_as_float(w[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < RUN; k++) {
-        const uint16_t b = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
-        v[k] = to_f(__builtin_bit_cast(T, b));
-      }
-    }
-    return;
+  widen<T, RUN>(v, load_words(p, n));
+}
+// Two floats rounded to nearest even, as one word.
+template <typename T>
+__device__ __forceinline__ uint32_t narrow_pair(float a, float b) {
+  if constexpr (__is_same(T, __half)) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+  } else {
+    return round_pair(f32x2{a, b});
   }
-#pragma unroll
-  for (int k = 0; k < RUN; k++) v[k] = k < n ? to_f(p[k]) : 0.0f;
 }
 
 template <typename T, int RUN>
@@ -201,9 +267,7 @@ __device__ __forceinline__ void store_run(T* p, const float (&v)[RUN], int64_t n
       for (int k = 0; k < RUN; k++) w[k] = __float_as_uint(v[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < RUN; k += 2)
-        w[k >> 1] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<T>(v[k])) |
-                    (uint32_t)__builtin_bit_cast(uint16_t, from_f<T>(v[k + 1])) << 16;
+      for (int k = 0; k < RUN; k += 2) w[k >> 1] = narrow_pair<T>(v[k], v[k + 1]);
     }
     ((Bytes16*)p)->v = w;
     return;
@@ -211,6 +275,37 @@ __device__ __forceinline__ void store_run(T* p, const float (&v)[RUN], int64_t n
 #pragma unroll
   for (int k = 0; k < RUN; k++)
     if (k < n) p[k] = from_f<T>(v[k]);
+}
+
+// The epilogue of RUN results v (and w, the up half) of row i at columns j..; n of them exist.
+template <typename T, int EPI, bool GATED, int ACT, int RUN>
+__device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_t j, int64_t n,
+                                         float (&v)[RUN], float (&w)[RUN], const float (&ex)[RUN]) {
+  T* out = (T*)p.out + i * p.out_row + j;
+#pragma unroll
+  for (int k = 0; k < RUN; k++) {
+    if (EPI == EPI_FORWARD) {
+      v[k] = GATED ? act_value<ACT>(v[k]) * w[k] : act_value<ACT>(v[k]) + ex[k];
+    } else if (EPI == EPI_DZ) {
+      float a;
+      const float s = act_both<ACT>(v[k], a);
+      v[k] = GATED ? ex[k] * w[k] * s : ex[k] * s;
+      if (GATED) w[k] = ex[k] * a;
+    }
+  }
+  store_run<T, RUN>(out, v, n);
+  if (EPI == EPI_DZ && GATED) store_run<T, RUN>(out + p.J, w, n);
+}
+
+// f(integral constant of the activation): one branch for a whole epilogue.
+template <int V> struct Const { static constexpr int value = V; };
+template <int EPI, typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+  if (EPI != EPI_FORWARD && EPI != EPI_DZ) return f(Const<GSR_ACT_NONE>());
+  if (act == GSR_ACT_RELU) f(Const<GSR_ACT_RELU>());
+  else if (act == GSR_ACT_GELU) f(Const<GSR_ACT_GELU>());
+  else if (act == GSR_ACT_SILU) f(Const<GSR_ACT_SILU>());
+  else f(Const<GSR_ACT_NONE>());
 }
 
 // One result in plain 32-bit arithmetic, r in [r0, r1) of each segment.
@@ -274,7 +369,6 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
   const int64_t lda = RCA ? p.a_i : p.a_r, ldb = RCB ? p.b_j : p.b_r;
   const uint32_t steps = (uint32_t)((r_end - r_begin + kDepth - 1) / kDepth);
   const uint32_t total = EPI == EPI_PLAIN ? steps * p.segments : steps;
-  const bool inside = i0 + BI <= p.I && j0 + kOut <= p.J;
 
   Chunk<T> ca[TA::kChunks], cb[TB::kChunks];
   auto load = [&](uint32_t it) {
@@ -286,14 +380,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
       b = (const T*)p.b[1];
     }
     const int64_t r0 = r_begin + (int64_t)it * kDepth;
-    constexpr int kSplit = GATED ? BJ / 2 : 0;
-    if (inside && r0 + kDepth <= r_end) {
-      TA::template load<true, 0>(ca, a, nullptr, lda, i0, p.I, r0, r_end);
-      TB::template load<true, kSplit>(cb, b, (const T*)p.b[1], ldb, j0, p.J, r0, r_end);
-    } else {
-      TA::template load<false, 0>(ca, a, nullptr, lda, i0, p.I, r0, r_end);
-      TB::template load<false, kSplit>(cb, b, (const T*)p.b[1], ldb, j0, p.J, r0, r_end);
-    }
+    TA::template load<0>(ca, a, nullptr, lda, i0, p.I, r0, r_end);
+    TB::template load<GATED ? BJ / 2 : 0>(cb, b, (const T*)p.b[1], ldb, j0, p.J, r0, r_end);
   };
   auto store = [&](int buffer) {
     char* s = lds + buffer * (TA::kBytes + TB::kBytes);
@@ -318,17 +406,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
         s16x8 a[kPlanes];
 #pragma unroll
         for (int q = 0; q < kPlanes; q++) a[q] = TA::read(sa + q * TA::kPlaneBytes, wi * NI + u, kk);
-        if constexpr (kPlanes == 1) {
 #pragma unroll
-          for (int t = 0; t < NJ; t++) acc[u][t] = mfma<T>(b[t][0], a[0], acc[u][t]);
-        } else {
-          // smallest products first; consecutive instructions work on different results
-          constexpr int kA[6] = {2, 0, 1, 1, 0, 0}, kB[6] = {0, 2, 1, 0, 1, 0};
+        for (int k = 0; k < Parts<kPlanes>::kProducts; k++)  // consecutive ones work on different results
 #pragma unroll
-          for (int k = 0; k < 6; k++)
-#pragma unroll
-            for (int t = 0; t < NJ; t++) acc[u][t] = mfma<T>(b[t][kB[k]], a[kA[k]], acc[u][t]);
-        }
+          for (int t = 0; t < NJ; t++)
+            acc[u][t] = mfma<T>(b[t][Parts<kPlanes>::kB[k]], a[Parts<kPlanes>::kA[k]], acc[u][t]);
         if (EPI == EPI_PARTIAL && sums) {  // the bias gradient: the same rows times ones
           const short one = sizeof(T) == 2 && __is_same(T, __half) ? 0x3c00 : 0x3f80;
           const s16x8 ones = {one, one, one, one, one, one, one, one};
@@ -401,52 +483,36 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
     }
   }
   constexpr int kRuns = NJ * 4 / RUN / (GATED ? 2 : 1);
+  with_act<EPI>(p.act, [&](auto act) {
 #pragma unroll
-  for (int s = 0; s < kRuns; s++) {
-    const int64_t j = j0 + wj * (NJ * 16) + (kPaired ? 32 * s + 8 * q : 16 * s + 4 * q);
-    const int64_t n = p.J - j;
-    if (n <= 0) continue;
-    float bias[RUN] = {}, bias1[RUN] = {};
-    if (EPI == EPI_FORWARD || EPI == EPI_DZ) {
-      if (p.bias[0]) load_run<T, RUN>(bias, (const T*)p.bias[0] + j, n);
-      if (GATED && p.bias[1]) load_run<T, RUN>(bias1, (const T*)p.bias[1] + j, n);
-    }
-#pragma unroll
-    for (int u = 0; u < NI; u++) {
-      const int64_t i = i0 + (wi * NI + u) * 16 + m;
-      if (i >= p.I) continue;
-      float v[RUN], w[RUN], ex[RUN] = {};
-#pragma unroll
-      for (int k = 0; k < RUN; k++) {
-        v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4] + bias[k];
-        if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4] + bias1[k];
+    for (int s = 0; s < kRuns; s++) {
+      const int64_t j = j0 + wj * (NJ * 16) + (kPaired ? 32 * s + 8 * q : 16 * s + 4 * q);
+      const int64_t n = p.J - j;
+      if (n <= 0) continue;
+      float bias[RUN] = {}, bias1[RUN] = {};
+      if (EPI == EPI_FORWARD || EPI == EPI_DZ) {
+        if (p.bias[0]) load_run<T, RUN>(bias, (const T*)p.bias[0] + j, n);
+        if (GATED && p.bias[1]) load_run<T, RUN>(bias1, (const T*)p.bias[1] + j, n);
       }
-      if (EPI == EPI_PARTIAL) {
-        store_run<float, 4>(p.part + ((int64_t)at.split * p.I + i) * p.J + j, (const float(&)[4])v, n);
-        continue;
-      }
-      if ((EPI == EPI_FORWARD || EPI == EPI_DZ) && p.extra)
-        load_run<T, RUN>(ex, (const T*)p.extra + i * p.extra_row + j, n);
-      T* out = (T*)p.out + i * p.out_row + j;
-      if (EPI == EPI_FORWARD) {
 #pragma unroll
-        for (int k = 0; k < RUN; k++) v[k] = GATED ? act_value(v[k], p.act) * w[k] : act_value(v[k], p.act) + ex[k];
-      } else if (EPI == EPI_DZ) {
+      for (int u = 0; u < NI; u++) {
+        const int64_t i = i0 + (wi * NI + u) * 16 + m;
+        if (i >= p.I) continue;
+        float v[RUN], w[RUN], ex[RUN] = {};
 #pragma unroll
         for (int k = 0; k < RUN; k++) {
-          if (GATED) {
-            const float d = ex[k] * act_value(v[k], p.act);
-            v[k] = ex[k] * w[k] * act_slope(v[k], p.act);
-            w[k] = d;
-          } else {
-            v[k] = ex[k] * act_slope(v[k], p.act);
-          }
+          v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4] + bias[k];
+          if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4] + bias1[k];
         }
-        if (GATED) store_run<T, RUN>(out + p.J, w, n);
+        if constexpr (EPI == EPI_PARTIAL) {
+          store_run<float, RUN>(p.part + ((int64_t)at.split * p.I + i) * p.J + j, v, n);
+        } else {
+          if (EPI != EPI_PLAIN && p.extra) load_run<T, RUN>(ex, (const T*)p.extra + i * p.extra_row + j, n);
+          epilogue<T, EPI, GATED, decltype(act)::value, RUN>(p, i, j, n, v, w, ex);
+        }
       }
-      store_run<T, RUN>(out, v, n);
     }
-  }
+  });
 }
 
 template <typename T, bool RCA, bool RCB, int EPI, bool GATED, int BI, int WI, int BJ, int WJ>
@@ -479,28 +545,10 @@ int launch_gated(const ProductArgs& p, hipStream_t stream) {
 }
 
 // What gsr_linear.hip needs of each type (gsr_linear_f32.hip, _f16.hip, _bf16.hip).
-template <typename T> int product_forward(const ProductArgs& p, bool gated, hipStream_t s);
-template <typename T> int product_dz(const ProductArgs& p, bool gated, hipStream_t s);
-template <typename T> int product_dx(const ProductArgs& p, hipStream_t s);
+template <typename T> size_t product_scratch(int64_t I, int64_t J, int64_t R, bool gated);
+template <typename T> int product_forward(const ProductArgs& p, bool gated, char* scratch, hipStream_t s);
+template <typename T> int product_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s);
+template <typename T> int product_dx(const ProductArgs& p, char* scratch, hipStream_t s);
 template <typename T> int product_dw(const ProductArgs& p, int64_t splits, hipStream_t s);
-
-#define GSR_PRODUCTS(T)                                                                              \
-  template <> int product_forward<T>(const ProductArgs& p, bool gated, hipStream_t s) {              \
-    if (gated) return launch_gated<T, EPI_FORWARD>(p, s);                                            \
-    return p.a_r == 1 ? launch_linear<T, true, true, EPI_FORWARD>(p, 1, s)                           \
-                      : launch_linear<T, false, true, EPI_FORWARD>(p, 1, s);                         \
-  }                                                                                                  \
-  template <> int product_dz<T>(const ProductArgs& p, bool gated, hipStream_t s) {                   \
-    if (gated) return launch_gated<T, EPI_DZ>(p, s);                                                 \
-    return p.a_r == 1 ? launch_linear<T, true, true, EPI_DZ>(p, 1, s)                                \
-                      : launch_linear<T, false, true, EPI_DZ>(p, 1, s);                              \
-  }                                                                                                  \
-  template <> int product_dx<T>(const ProductArgs& p, hipStream_t s) {                               \
-    return launch_linear<T, true, false, EPI_PLAIN>(p, 1, s);                                        \
-  }                                                                                                  \
-  template <> int product_dw<T>(const ProductArgs& p, int64_t splits, hipStream_t s) {               \
-    return p.b_j == 1 ? launch_linear<T, false, false, EPI_PARTIAL>(p, splits, s)                    \
-                      : launch_linear<T, false, true, EPI_PARTIAL>(p, splits, s);                    \
-  }
 
 }  // namespace gsr

@@ -1,0 +1,322 @@
+// gsr_strip.h -- the product of many rows with few inputs (a head's layers: K <= 256, a view's
+// pixels as rows): a wave keeps its rows of x in registers and walks along the outputs.
+//
+// At these widths a tile of C has only a few steps along K, so a tiled kernel spends its time
+// filling and draining pipelines.  Here a wave loads all of its 16 NI rows at once, straight into
+// the matrix instruction's operand layout (every byte of x is read once, and all of a workgroup's
+// reads are in flight together).  The weights are first written out once as the images that LDS is
+// to hold (16-bit parts, padded with zeros to whole tiles, rows in reading order): a tile's image
+// goes to LDS by direct loads without passing registers or needing bounds, two tiles ahead, so that
+// neither it nor the stores of finished results are waited for.
+#pragma once
+#include "gsr_product.h"
+
+namespace gsr {
+
+// kRows rows of weights in a tile, kWaves waves of 16 kNI rows of x, for up to 32 KS inputs: three
+// tiles of two or three workgroups fit the LDS of a CU (of one with twice the waves, gated: a tile
+// has the rows of both halves).
+template <typename T, int KS, bool GATED> struct Strip {
+  static constexpr int kNI = sizeof(T) == 4 && KS > 4 ? 1 : 2;  // three parts of x fill the registers
+  static constexpr int kWaves = GATED && sizeof(T) == 4 && KS > 6 ? 8 : 4;
+  static constexpr int kRows = sizeof(T) == 4 ? (KS > 6 && !GATED ? 16 : 32) : 64;
+  static constexpr int kOut = GATED ? kRows / 2 : kRows;  // outputs of a tile
+  // Bytes of a row: the 32 of padding turn it by two of the 16 bank groups, so that the lanes that
+  // a 16-byte read takes together (0-3, 12-15, 20-23, 24-27 and so on) hit different ones.  The
+  // first rows' padding holds the tile's biases as floats, 8 to a row.
+  static constexpr int kRow = KS * 64 + 32;
+  static constexpr int kPlane = kRows * kRow;
+  static constexpr int kImage = (kPlane * Operand<T>::kPlanes + 1023) / 1024 * 1024;
+};
+
+// One thread per 8 weights: tile, row, chunk.
+template <typename T, bool GATED, int KS>
+__global__ __launch_bounds__(256) void image_kernel(ProductArgs p, char* images, uint32_t chunks) {
+  using S = Strip<T, KS, GATED>;
+  constexpr int LR = S::kRows, kOut = S::kOut;
+  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
+  if (id >= chunks) return;
+  const int at = id % (KS * 4), row = id / (KS * 4) % LR;
+  const uint32_t tile = id / (KS * 4 * LR);
+  const bool second = GATED && row >= kOut;
+  const int64_t j = (int64_t)tile * kOut + (second ? row - kOut : row);
+  const T* w = (const T*)p.b[second ? 1 : 0] + j * p.b_j;
+  char* image = images + (size_t)tile * S::kImage;
+  if (at == 0) {
+    const T* bias = (const T*)p.bias[second ? 1 : 0];
+    ((float*)(image + row / 8 * S::kRow + KS * 64))[row % 8] = bias && j < p.J ? to_f(bias[j]) : 0.0f;
+  }
+  Chunk<T> c;
+#pragma unroll
+  for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = u32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const int64_t r = at * 8 + e;
+    if (j >= p.J || r >= p.R) continue;
+    if constexpr (sizeof(T) == 4) c.w[e >> 2][e & 3] = ((const uint32_t*)w)[r * p.b_r];
+    else c.w[0][e >> 1] |= (uint32_t)((const uint16_t*)w)[r * p.b_r] << (16 * (e & 1));
+  }
+  // 16-bit results leave 8 at a time: the rows of a read are 4 + 4 + 4 + 4, 8 apart
+  const int place = sizeof(T) == 2 ? (row & ~31) + 16 * ((row >> 2) & 1) + 4 * ((row >> 3) & 3) + (row & 3) : row;
+  put_chunk<T>(image + place * S::kRow + at * 16, S::kPlane, c);
+}
+
+template <typename T, bool RCA, int EPI, bool GATED, int KS>
+__global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_kernel(
+    ProductArgs p, const char* images, uint32_t strips, uint32_t parts, uint32_t part_tiles) {
+  using S = Strip<T, KS, GATED>;
+  constexpr int kPlanes = Operand<T>::kPlanes, NI = S::kNI, kWaves = S::kWaves, kOut = S::kOut;
+  constexpr bool kPaired = sizeof(T) == 2;
+  constexpr int RUN = kPaired ? 8 : 4, NJ = S::kRows / 16, kRuns = kOut / 4 / RUN;
+  static_assert(kRuns >= 1 && NJ >= 1, "");
+  __shared__ __attribute__((aligned(1024))) char lds[2 * S::kImage];
+
+  const uint32_t each = gridDim.x >> 3, id = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  if (id >= strips * parts) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int m = lane & 15, q = lane >> 4;
+  const int K = (int)p.R;
+  const int64_t i0 = ((int64_t)(id / parts) * kWaves + wave) * (16 * NI);
+  const uint32_t tile0 = id % parts * part_tiles, all = (uint32_t)((p.J + kOut - 1) / kOut);
+  const uint32_t tile1 = tile0 + part_tiles < all ? tile0 + part_tiles : all;
+  if (tile0 >= tile1) return;
+  // Workgroups start at different tiles: rows of a power of two would otherwise have all of them
+  // write to the same few memory channels at a time.
+  const uint32_t count = tile1 - tile0, turn = id / parts % count;
+  auto tile_at = [&](uint32_t t) {
+    t = t < count ? t : count - 1;
+    return tile0 + (t + turn < count ? t + turn : t + turn - count);
+  };
+
+  // An image into LDS, 1 KB per instruction; every wave issues as many (the last KB more than once).
+  constexpr int kFetches = (S::kImage / 1024 + kWaves - 1) / kWaves;
+  auto fetch = [&](uint32_t t, uint32_t buffer) {
+    const char* src = images + (size_t)tile_at(t) * S::kImage + lane * 16;
+    char* to = lds + buffer * S::kImage;
+#pragma unroll
+    for (int u = 0; u < kFetches; u++) {
+      const int unit = u * kWaves + wave, at = (unit < S::kImage / 1024 ? unit : S::kImage / 1024 - 1) * 1024;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + at),
+                                       (__attribute__((address_space(3))) void*)(to + at), 16, 0, 0);
+    }
+  };
+  auto row_of = [&](int u) {  // a row past the last is the last one again: its results are not stored
+    const int64_t i = i0 + u * 16 + m;
+    return i < p.I ? i : p.I - 1;
+  };
+  auto column_of = [&](int s) { return kPaired ? 32 * s + 8 * q : 16 * s + 4 * q; };
+  auto load_extra = [&](u32x4 (&ex)[NI][kRuns], uint32_t t) {
+    const int64_t j0 = (int64_t)tile_at(t) * kOut;
+    const bool whole = j0 + kOut <= p.J;
+#pragma unroll
+    for (int u = 0; u < NI; u++)
+#pragma unroll
+      for (int s = 0; s < kRuns; s++) {
+        const T* e = (const T*)p.extra + row_of(u) * p.extra_row;
+        ex[u][s] = whole ? ((const Bytes16*)(e + j0 + column_of(s)))->v : load_tail_words(e, j0 + column_of(s), p.J);
+      }
+  };
+
+  fetch(0, 0);
+  s16x8 a[NI][KS][kPlanes];
+#pragma unroll
+  for (int u = 0; u < NI; u++) {
+    const int64_t i = row_of(u);
+#pragma unroll
+    for (int kk = 0; kk < KS; kk++) {
+      const int k = kk * 32 + q * 8;
+      Chunk<T> c = {};
+      if (RCA) {
+        const T* x = (const T*)p.a + i * p.a_i;
+        if (kk * 32 + 32 <= K) c = load_whole(x + k);
+        else if (kk * 32 < K) c = load_tail(x, k, 1, K);
+      } else if (kk * 32 < K) {
+        c = load_tail((const T*)p.a + i, k, p.a_r, K);
+      }
+      split_chunk<T>(a[u][kk], c);
+    }
+  }
+  u32x4 ex[NI][kRuns] = {}, ex_next[NI][kRuns] = {};
+  if (p.extra) load_extra(ex, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  const bool rows_in = i0 + 16 * NI <= p.I;
+
+  for (uint32_t step = 0, buffer = 0; step < count; step++) {
+    // every wave's part of this image is in LDS, and everyone has left the image before it
+    barrier();
+    fetch(step + 1, buffer ^ 1);
+    if (p.extra) load_extra(ex_next, step + 1);
+    const int64_t j0 = (int64_t)tile_at(step) * kOut;
+    const char* image = lds + buffer * S::kImage;
+    f32x4 acc[NI][NJ] = {};
+    // the operands of kAhead reads are on their way while the products of the one before are formed
+    constexpr int kReads = KS * NJ, kAhead = kReads * kPlanes < 8 ? kReads : 8 / kPlanes;
+    s16x8 b[kAhead][kPlanes];
+    auto read = [&](int n) {
+      const int kk = n / NJ, t = n % NJ;
+#pragma unroll
+      for (int z = 0; z < kPlanes; z++)
+        b[n % kAhead][z] = *(const s16x8*)(image + z * S::kPlane + (16 * t + m) * S::kRow + (kk * 4 + q) * 16);
+    };
+#pragma unroll
+    for (int n = 0; n < kAhead; n++) read(n);
+#pragma unroll
+    for (int n = 0; n < kReads; n++) {
+      const int kk = n / NJ, t = n % NJ;
+#pragma unroll
+      for (int k = 0; k < Parts<kPlanes>::kProducts; k++)
+#pragma unroll
+        for (int u = 0; u < NI; u++)
+          acc[u][t] = mfma<T>(b[n % kAhead][Parts<kPlanes>::kB[k]], a[u][kk][Parts<kPlanes>::kA[k]], acc[u][t]);
+      if (n + kAhead < kReads) read(n + kAhead);
+      __builtin_amdgcn_sched_barrier(0);  // keeps this order
+    }
+    if constexpr (sizeof(T) == 4) {
+      float odd = 0.0f;  // stays 0 while every result is finite
+#pragma unroll
+      for (int u = 0; u < NI; u++)
+#pragma unroll
+        for (int t = 0; t < NJ; t++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) odd = fmaf(acc[u][t][v], 0.0f, odd);
+      if (odd != 0.0f) {
+#pragma unroll
+        for (int u = 0; u < NI; u++)
+#pragma unroll
+          for (int t = 0; t < NJ; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+              const int row = t * 16 + 4 * q + v;
+              const bool second = GATED && row >= kOut;
+              const int64_t i = i0 + u * 16 + m, j = j0 + (second ? row - kOut : row);
+              if (i < p.I && j < p.J && !(fabsf(acc[u][t][v]) <= 3.4e38f))
+                acc[u][t][v] = exact_sum((const float*)p.a, p.a_i, p.a_r, (const float*)p.b[second ? 1 : 0],
+                                         nullptr, p.b_j, p.b_r, 1, 0, i, j, 0, K);
+            }
+      }
+    }
+    const bool whole = rows_in && j0 + kOut <= p.J;
+    auto finish = [&](auto act, auto full) {
+      constexpr bool FULL = decltype(full)::value;
+#pragma unroll
+      for (int s = 0; s < kRuns; s++) {
+        const int64_t j = j0 + column_of(s), n = FULL ? RUN : p.J - j;
+        if (!FULL && n <= 0) continue;
+        float bias[RUN] = {}, bias1[RUN] = {};
+        auto load_bias = [&](float (&v)[RUN], int row) {
+          const f32x4* w = (const f32x4*)(image + row / 8 * S::kRow + KS * 64 + row % 8 * 4);
+#pragma unroll
+          for (int k = 0; k < RUN; k++) v[k] = w[k / 4][k % 4];
+        };
+        if (EPI != EPI_PLAIN) load_bias(bias, column_of(s));
+        if (EPI != EPI_PLAIN && GATED) load_bias(bias1, kOut + column_of(s));
+#pragma unroll
+        for (int u = 0; u < NI; u++) {
+          const int64_t i = i0 + u * 16 + m;
+          if (!FULL && i >= p.I) continue;
+          float v[RUN], w[RUN], e[RUN];
+          widen<T, RUN>(e, ex[u][s]);
+#pragma unroll
+          for (int k = 0; k < RUN; k++) {
+            v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4] + bias[k];
+            if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4] + bias1[k];
+          }
+          epilogue<T, EPI, GATED, decltype(act)::value, RUN>(p, i, j, n, v, w, e);
+        }
+      }
+    };
+    with_act<EPI>(p.act, [&](auto act) {
+      if (whole) finish(act, Const<1>());
+      else finish(act, Const<0>());
+    });
+    // This wave's part of the next image has to be there.  It was asked for before the stores of
+    // this tile, which may go on: a whole tile has kStores of them.
+    constexpr int kStores = NI * kRuns * (EPI == EPI_DZ && GATED ? 2 : 1);
+    if (whole) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < NI; u++)
+#pragma unroll
+      for (int s = 0; s < kRuns; s++) ex[u][s] = ex_next[u][s];
+    buffer ^= 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing arrives in LDS that is another's
+}
+
+template <typename T, bool GATED, int KS>
+size_t image_bytes(int64_t J) {
+  using S = Strip<T, KS, GATED>;
+  return (size_t)((J + S::kOut - 1) / S::kOut) * S::kImage;
+}
+
+template <typename T, bool RCA, int EPI, bool GATED, int KS>
+int launch_strip(const ProductArgs& p, char* scratch, hipStream_t stream) {
+  using S = Strip<T, KS, GATED>;
+  constexpr int kOut = S::kOut, kBlock = S::kWaves * 16 * S::kNI;
+  const int64_t strips = (p.I + kBlock - 1) / kBlock, tiles = (p.J + kOut - 1) / kOut;
+  const int64_t chunks = tiles * S::kRows * KS * 4;
+  // too few strips to give every CU two workgroups: several workgroups share one's outputs
+  int64_t parts = strips >= 512 ? 1 : (512 + strips - 1) / strips;
+  if (parts > tiles) parts = tiles;
+  const int64_t part_tiles = (tiles + parts - 1) / parts;
+  if (strips > 0x7ffffff0 / parts || chunks > 0x7fffffff) return 1;
+  hipLaunchKernelGGL((image_kernel<T, GATED, KS>), dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, stream, p,
+                     scratch, (uint32_t)chunks);
+  hipLaunchKernelGGL((strip_kernel<T, RCA, EPI, GATED, KS>), dim3((uint32_t)((strips * parts + 7) / 8 * 8)),
+                     dim3(64 * S::kWaves), 0, stream, p, (const char*)scratch, (uint32_t)strips, (uint32_t)parts,
+                     (uint32_t)part_tiles);
+  return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+
+// Strips for up to 256 inputs and enough rows that every CU has one.
+inline bool takes_strips(int64_t I, int64_t R) { return R <= 256 && I >= 4096; }
+
+// f(integral constant KS) for R inputs.
+template <typename F>
+auto with_steps(int64_t R, F f) {
+  if (R <= 32) return f(Const<1>());
+  if (R <= 64) return f(Const<2>());
+  if (R <= 128) return f(Const<4>());
+  if (R <= 192) return f(Const<6>());
+  return f(Const<8>());
+}
+
+template <typename T, bool RCA, int EPI, bool GATED>
+int launch_strips(const ProductArgs& p, char* scratch, hipStream_t s) {
+  return with_steps(p.R, [&](auto ks) { return launch_strip<T, RCA, EPI, GATED, decltype(ks)::value>(p, scratch, s); });
+}
+
+template <typename T, int EPI>
+int forward_or_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) {
+  const bool strips = takes_strips(p.I, p.R);
+  if (gated) return strips ? launch_strips<T, true, EPI, true>(p, scratch, s) : launch_gated<T, EPI>(p, s);
+  if (p.a_r == 1)
+    return strips ? launch_strips<T, true, EPI, false>(p, scratch, s) : launch_linear<T, true, true, EPI>(p, 1, s);
+  return strips ? launch_strips<T, false, EPI, false>(p, scratch, s) : launch_linear<T, false, true, EPI>(p, 1, s);
+}
+
+#define GSR_PRODUCTS(T)                                                                              \
+  template <> size_t product_scratch<T>(int64_t I, int64_t J, int64_t R, bool gated) {               \
+    if (!takes_strips(I, R)) return 0;                                                               \
+    return with_steps(R, [&](auto ks) {                                                              \
+      constexpr int KS = decltype(ks)::value;                                                        \
+      return gated ? image_bytes<T, true, KS>(J) : image_bytes<T, false, KS>(J);                     \
+    });                                                                                              \
+  }                                                                                                  \
+  template <> int product_forward<T>(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) { \
+    return forward_or_dz<T, EPI_FORWARD>(p, gated, scratch, s);                                      \
+  }                                                                                                  \
+  template <> int product_dz<T>(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) {    \
+    return forward_or_dz<T, EPI_DZ>(p, gated, scratch, s);                                           \
+  }                                                                                                  \
+  template <> int product_dx<T>(const ProductArgs& p, char* scratch, hipStream_t s) {                \
+    if (p.segments == 1 && takes_strips(p.I, p.R))                                                   \
+      return launch_strips<T, true, EPI_PLAIN, false>(p, scratch, s);                                \
+    return launch_linear<T, true, false, EPI_PLAIN>(p, 1, s);                                        \
+  }                                                                                                  \
+  template <> int product_dw<T>(const ProductArgs& p, int64_t splits, hipStream_t s) {               \
+    return p.b_j == 1 ? launch_linear<T, false, false, EPI_PARTIAL>(p, splits, s)                    \
+                      : launch_linear<T, false, true, EPI_PARTIAL>(p, splits, s);                    \
+  }
+
+}  // namespace gsr

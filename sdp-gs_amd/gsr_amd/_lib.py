@@ -278,7 +278,10 @@ def load():
         # include/gsr_linear.h
         L.gsr_linear.restype = _i
         L.gsr_linear.argtypes = [_i, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i,
-                                 _p, _i64, _p]
+                                 _p, _i64, _p, _p]
+        for n in ("gsr_linear_scratch_bytes", "gsr_gated_scratch_bytes"):
+            getattr(L, n).restype = _sz
+            getattr(L, n).argtypes = [_i, _i64, _i64, _i64]
         L.gsr_linear_backward_scratch_bytes.restype = _sz
         L.gsr_linear_backward_scratch_bytes.argtypes = [_i, _i64, _i64, _i64, _i, _i]
         L.gsr_linear_backward.restype = _i
@@ -286,7 +289,7 @@ def load():
                                           _p, _i64, _p, _p, _p, _p, _p]
         L.gsr_gated.restype = _i
         L.gsr_gated.argtypes = [_i, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i, _p, _i64,
-                                _p]
+                                _p, _p]
         L.gsr_gated_backward_scratch_bytes.restype = _sz
         L.gsr_gated_backward_scratch_bytes.argtypes = [_i, _i64, _i64, _i64, _i]
         L.gsr_gated_backward.restype = _i

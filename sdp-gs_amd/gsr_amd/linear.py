@@ -104,11 +104,13 @@ class _Linear(torch.autograd.Function):
         r = None if residual is None else _rows(residual, N)
         y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
         if M:
+            L = _lib.load()
+            scratch = _scratch(L.gsr_linear_scratch_bytes(DTYPES[x.dtype], M, K, N), x.device)
             with _lib.on_device(x.device):
-                _check(_lib.load().gsr_linear(
+                _check(L.gsr_linear(
                     DTYPES[x.dtype], M, K, N, xm.data_ptr(), x_row, x_col, w.data_ptr(),
                     _row_stride(w), _ptr(b), _ptr(r), 0 if r is None else _row_stride(r), act,
-                    y.data_ptr(), N, _lib.raw_stream(x.device)), "gsr_linear")
+                    y.data_ptr(), N, scratch.data_ptr(), _lib.raw_stream(x.device)), "gsr_linear")
         ctx.save_for_backward(xm, w, b)
         ctx.args = (x.shape, x_row, x_col, act)
         return y
@@ -150,11 +152,13 @@ class _Gated(torch.autograd.Function):
         bu = None if up_bias is None else up_bias.detach().contiguous()
         h = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
         if M:
+            L = _lib.load()
+            scratch = _scratch(L.gsr_gated_scratch_bytes(DTYPES[x.dtype], M, K, N), x.device)
             with _lib.on_device(x.device):
-                _check(_lib.load().gsr_gated(
+                _check(L.gsr_gated(
                     DTYPES[x.dtype], M, K, N, xm.data_ptr(), _row_stride(xm), wg.data_ptr(),
                     wu.data_ptr(), _row_stride(wg), _ptr(bg), _ptr(bu), act, h.data_ptr(), N,
-                    _lib.raw_stream(x.device)), "gsr_gated")
+                    scratch.data_ptr(), _lib.raw_stream(x.device)), "gsr_gated")
         ctx.save_for_backward(xm, wg, wu, bg, bu)
         ctx.args = (x.shape, act)
         return h
