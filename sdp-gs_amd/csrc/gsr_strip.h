@@ -9,7 +9,7 @@
 // goes to LDS by direct loads without passing registers or needing bounds, two tiles ahead, so that
 // neither it nor the stores of finished results are waited for.
 #pragma once
-#include "gsr_product.h"
+#include "gsr_rows.h"
 
 namespace gsr {
 
@@ -289,6 +289,8 @@ int launch_strips(const ProductArgs& p, char* scratch, hipStream_t s) {
 template <typename T, int EPI>
 int forward_or_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) {
   const bool strips = takes_strips(p.I, p.R);
+  if constexpr (EPI == EPI_FORWARD)
+    if (takes_rows(p)) return gated ? launch_rows<T, EPI, true>(p, s) : launch_rows<T, EPI, false>(p, s);
   if (gated) return strips ? launch_strips<T, true, EPI, true>(p, scratch, s) : launch_gated<T, EPI>(p, s);
   if (p.a_r == 1)
     return strips ? launch_strips<T, true, EPI, false>(p, scratch, s) : launch_linear<T, true, true, EPI>(p, 1, s);

@@ -64,7 +64,6 @@ def _weight_sizes(x, weight, name):
 
 def _rows(t, n):
     """t [..., n] as a [M, n] matrix whose rows are contiguous (a copy only if it has to be)."""
-    t = t.detach()
     m = t.reshape(-1, n) if t.dim() != 2 else t
     if (n > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < n):
         m = m.contiguous()
@@ -78,7 +77,6 @@ def _row_stride(m):
 
 def _x_matrix(x, K):
     """x as (matrix, row stride, column stride): channel-major memory is taken as it lies."""
-    x = x.detach()
     if x.dim() == 2 and K > 1 and x.shape[0] > 1 and x.stride(0) == 1 and x.stride(1) >= x.shape[0]:
         return x, 1, int(x.stride(1))
     m = _rows(x, K)
@@ -93,6 +91,10 @@ def _scratch(nbytes, device):
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
@@ -100,7 +102,7 @@ class _Linear(torch.autograd.Function):
         xm, x_row, x_col = _x_matrix(x, K)
         M = xm.shape[0]
         w = _rows(weight, K)
-        b = None if bias is None else bias.detach().contiguous()
+        b = None if bias is None else bias.contiguous()
         r = None if residual is None else _rows(residual, N)
         y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
         if M:
@@ -111,8 +113,9 @@ class _Linear(torch.autograd.Function):
                     DTYPES[x.dtype], M, K, N, xm.data_ptr(), x_row, x_col, w.data_ptr(),
                     _row_stride(w), _ptr(b), _ptr(r), 0 if r is None else _row_stride(r), act,
                     y.data_ptr(), N, scratch.data_ptr(), _lib.raw_stream(x.device)), "gsr_linear")
-        ctx.save_for_backward(xm, w, b)
-        ctx.args = (x.shape, x_row, x_col, act)
+        if ctx is not None:
+            ctx.save_for_backward(xm, w, b)
+            ctx.args = (x.shape, x_row, x_col, act)
         return y
 
     @staticmethod
@@ -148,8 +151,8 @@ class _Gated(torch.autograd.Function):
         wg, wu = _rows(gate, K), _rows(up, K)
         if _row_stride(wg) != _row_stride(wu):
             wg, wu = wg.contiguous(), wu.contiguous()
-        bg = None if gate_bias is None else gate_bias.detach().contiguous()
-        bu = None if up_bias is None else up_bias.detach().contiguous()
+        bg = None if gate_bias is None else gate_bias.contiguous()
+        bu = None if up_bias is None else up_bias.contiguous()
         h = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
         if M:
             L = _lib.load()
@@ -159,8 +162,9 @@ class _Gated(torch.autograd.Function):
                     DTYPES[x.dtype], M, K, N, xm.data_ptr(), _row_stride(xm), wg.data_ptr(),
                     wu.data_ptr(), _row_stride(wg), _ptr(bg), _ptr(bu), act, h.data_ptr(), N,
                     scratch.data_ptr(), _lib.raw_stream(x.device)), "gsr_gated")
-        ctx.save_for_backward(xm, wg, wu, bg, bu)
-        ctx.args = (x.shape, act)
+        if ctx is not None:
+            ctx.save_for_backward(xm, wg, wu, bg, bu)
+            ctx.args = (x.shape, act)
         return h
 
     @staticmethod
@@ -196,6 +200,8 @@ def fused_linear(x, weight, bias=None, *, activation="none", residual=None):
     N, K = _weight_sizes(x, weight, "weight")
     _checked(x, [("x", x, x.shape[:-1] + (K,)), ("weight", weight, (N, K)), ("bias", bias, (N,)),
                  ("residual", residual, x.shape[:-1] + (N,))], activation)
+    if not _wants_grad(x, weight, bias, residual):
+        return _Linear.forward(None, x, weight, bias, residual, ACTIVATIONS[activation])
     return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation])
 
 
@@ -206,4 +212,7 @@ def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, act
     _checked(x, [("x", x, x.shape[:-1] + (K,)), ("gate_weight", gate_weight, (N, K)),
                  ("up_weight", up_weight, (N, K)), ("gate_bias", gate_bias, (N,)),
                  ("up_bias", up_bias, (N,))], activation)
+    if not _wants_grad(x, gate_weight, up_weight, gate_bias, up_bias):
+        return _Gated.forward(None, x, gate_weight, up_weight, gate_bias, up_bias,
+                              ACTIVATIONS[activation])
     return _Gated.apply(x, gate_weight, up_weight, gate_bias, up_bias, ACTIVATIONS[activation])

@@ -50,47 +50,56 @@ def _dense(t):
     return True
 
 
-def _norm_args(tensors, norm_type):
-    """The tensors that hold elements, checked: (tensors, norm code)."""
+def _norm_code(norm_type):
     if isinstance(norm_type, str) or float(norm_type) not in _NORMS:
         raise ValueError(f"norm_type must be 1, 2 or inf, not {norm_type!r}")
+    return _NORMS[float(norm_type)]
+
+
+def _nonempty(tensors):
+    """The tensors that hold elements, each checked."""
     kept = []
+    device = tensors[0].device if tensors else None
     for t in tensors:
-        if t.layout != torch.strided:
+        if t.layout is not torch.strided:
             raise RuntimeError("gradient norm: sparse gradients are not supported")
         if t.dtype not in _DTYPES:
             raise ValueError(f"gradient norm: float32, float16 or bfloat16 expected, not {t.dtype}")
         if not t.is_cuda:
             raise RuntimeError("gradient norm: HIP tensors only (no CPU path)")
-        if t.device != tensors[0].device:
+        if t.device != device:
             raise ValueError("gradient norm: every gradient must be on one device")
         if t.numel():
             kept.append(t)
-    return kept, _NORMS[float(norm_type)]
+    return kept
 
 
-def _c_tensors(ts):
-    n = len(ts)
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]),
-            (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
-            (ctypes.c_int * n)(*[_DTYPES[t.dtype] for t in ts]))
+class _CTensors:
+    """The tensors as the C entries take them; one with gaps between its elements as a copy."""
+
+    def __init__(self, tensors):
+        self.tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
+        self.n = n = len(tensors)
+        self.pointers = [t.data_ptr() for t in self.tensors]
+        self.args = ((ctypes.c_void_p * n)(*self.pointers),
+                     (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
+                     (ctypes.c_int * n)(*[_DTYPES[t.dtype] for t in tensors]))
+        self.device = tensors[0].device
+        self.scratch = torch.empty(int(_lib.load().gsr_grad_norm_scratch_bytes(n)),
+                                   dtype=torch.uint8, device=self.device)
+        self.norm = torch.empty((), dtype=torch.float32, device=self.device)
 
 
 def _norm_and_scale(tensors, norm_code, max_norm, scale=None):
     """gsr_grad_norm on the current stream: the norm (and `scale`, a one-float tensor)."""
-    dev = tensors[0].device
-    ts = [t.detach() if _dense(t) else t.detach().contiguous() for t in tensors]
-    ptrs, numel, kinds = _c_tensors(ts)
-    L = _lib.load()
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    scratch = torch.empty(int(L.gsr_grad_norm_scratch_bytes(len(ts))), dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        rc = L.gsr_grad_norm(len(ts), ptrs, numel, kinds, norm_code, float(max_norm),
-                             norm.data_ptr(), None if scale is None else scale.data_ptr(),
-                             scratch.data_ptr(), _lib.raw_stream(dev))
+    c = _CTensors(tensors)
+    with _lib.on_device(c.device):
+        rc = _lib.load().gsr_grad_norm(c.n, *c.args, norm_code, float(max_norm), c.norm.data_ptr(),
+                                       None if scale is None else scale.data_ptr(),
+                                       c.scratch.data_ptr(), _lib.raw_stream(c.device))
     if rc != 0:
         raise RuntimeError(f"gsr_grad_norm failed with status {rc}")
-    return norm
+    return c.norm
 
 
 @torch.no_grad()
@@ -99,24 +108,33 @@ def grad_norm(tensors, norm_type=2.0):
     device (not synchronised).  Any number of tensors, of mixed types, strides and sizes; sums in
     64 bits, the same tensors give the same bits.  No tensors (or only empty ones): 0."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    kept, code = _norm_args(tensors, norm_type)
+    code, kept = _norm_code(norm_type), _nonempty(tensors)
     if not kept:
         return torch.zeros((), device=tensors[0].device if tensors else "cpu")
     return _norm_and_scale(kept, code, math.inf)
 
 
-def _refuse_overlap(grads):
+def _refuse_overlap(grads, c):
     """Two workgroups may not scale the same memory.  Gradients with gaps are scaled in copies, so
     only their overlap with one that is scaled in place counts."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(
-        (n - 1) * s for n, s in zip(t.shape, t.stride()))), _dense(t)) for t in grads)
+    spans = []
+    for t, own, start in zip(grads, c.tensors, c.pointers):
+        if t is own:
+            spans.append((start, start + t.numel() * t.element_size(), True))
+            continue
+        if 0 in [s for n, s in zip(t.shape, t.stride()) if n > 1]:
+            raise ValueError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        spans.append((t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size(), False))
+    spans.sort()
     end_dense = end_any = 0
     for start, end, dense in spans:
         if start < (end_any if dense else end_dense):
             raise ValueError("clip_grad_norm_: two gradients share memory (the same one twice?)")
-        end_any = max(end_any, end)
-        if dense:
-            end_dense = max(end_dense, end)
+        if end > end_any:
+            end_any = end
+        if dense and end > end_dense:
+            end_dense = end
 
 
 @torch.no_grad()
@@ -129,34 +147,27 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be at least 0, not {max_norm}")
-    grads = [p.grad for p in parameters if p.grad is not None]
-    kept, code = _norm_args(grads, norm_type)
+    code = _norm_code(norm_type)
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    kept = _nonempty(grads)
     if not kept:
         return torch.zeros((), device=grads[0].device if grads else "cpu")
-    for t in kept:
-        if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
-            raise ValueError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
-    _refuse_overlap(kept)
+    c = _CTensors(kept)
+    _refuse_overlap(kept, c)
     if error_if_nonfinite:
         norm = _norm_and_scale(kept, code, math.inf)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"The total norm of order {norm_type} is non-finite, so it cannot "
                                "be clipped")
-    dev = kept[0].device
-    ts = [t.detach() if _dense(t) else t.detach().contiguous() for t in kept]
-    ptrs, numel, kinds = _c_tensors(ts)
-    L = _lib.load()
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    scratch = torch.empty(int(L.gsr_grad_norm_scratch_bytes(len(ts))), dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        rc = L.gsr_clip_grads(len(ts), ptrs, numel, kinds, code, max_norm, norm.data_ptr(),
-                              scratch.data_ptr(), _lib.raw_stream(dev))
+    with _lib.on_device(c.device):
+        rc = _lib.load().gsr_clip_grads(c.n, *c.args, code, max_norm, c.norm.data_ptr(),
+                                        c.scratch.data_ptr(), _lib.raw_stream(c.device))
     if rc != 0:
         raise RuntimeError(f"gsr_clip_grads failed with status {rc}")
-    for t, c in zip(kept, ts):
-        if t.data_ptr() != c.data_ptr():  # a gradient with gaps: its scaled copy goes back
-            t.copy_(c)
-    return norm
+    for t, own in zip(kept, c.tensors):
+        if t is not own:  # a gradient with gaps: its scaled copy goes back
+            t.copy_(own)
+    return c.norm
 
 
 class FusedAdam(torch.optim.Adam):
@@ -226,10 +237,10 @@ class FusedAdam(torch.optim.Adam):
         parameter (dim 0), end_rows(h) finishes.  The row ranges must cover every row exactly
         once; the result is bitwise the one of step() (the update is elementwise)."""
         self._resolve_pending()
-        kept, norm_code = [], 2
+        kept = []
         if self.max_grad_norm is not None:  # refused before any step count advances
-            kept, norm_code = _norm_args([p.grad for group in self.param_groups
-                                          for p in group["params"] if p.grad is not None], 2.0)
+            kept = _nonempty([p.grad for group in self.param_groups for p in group["params"]
+                              if p.grad is not None])
         batches = {}
         for group in self.param_groups:
             beta1, beta2 = group["betas"]
@@ -286,7 +297,7 @@ class FusedAdam(torch.optim.Adam):
         scale = None
         if kept:
             scale = torch.empty(1, dtype=torch.float32, device=kept[0].device)
-            self.grad_norm = _norm_and_scale(kept, norm_code, self.max_grad_norm, scale)
+            self.grad_norm = _norm_and_scale(kept, _NORMS[2.0], self.max_grad_norm, scale)
         return {"batches": batches, "skips": skips, "states": states, "issued": False,
                 "scale": scale}
 
