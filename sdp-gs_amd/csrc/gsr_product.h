@@ -33,6 +33,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // 16 bytes at any address: operands may start anywhere (a slice, an odd row length)
 struct __attribute__((packed, aligned(1))) Bytes16 { u32x4 v; };
 
+template <int V> struct Const { static constexpr int value = V; };
+
 template <typename T> struct Operand {
   static constexpr int kPlanes = 1, kDepth = 64, kBuffers = 2, kRaw = 1;  // kRaw: 16-byte words per 8 elements
 };
@@ -89,6 +91,23 @@ __device__ __forceinline__ Chunk<T> load_tail(const T* row, int64_t k, int64_t s
   }
   return c;
 }
+// The same from whole words: up to 7 elements past the row's end are read, which has to be memory
+// of the tensor (there are rows after it).
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_masked(const T* row, int64_t k, int64_t n) {
+  Chunk<T> c = load_whole(row + (k < n ? k : 0));
+  const int64_t left = n - k;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) c.w[e >> 2][e & 3] = e < left ? c.w[e >> 2][e & 3] : 0u;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) c.w[0][e] &= 2 * e + 1 < left ? ~0u : 2 * e < left ? 0xffffu : 0u;
+  }
+  return c;
+}
+constexpr int kSpareRows = 8;  // with so many rows after it, a row may be read 7 elements too far
+
 // 16 bytes of a row of n elements from element k on; those past its end repeat its last.
 template <typename T>
 __device__ __forceinline__ u32x4 load_tail_words(const T* row, int64_t k, int64_t n) {
@@ -167,29 +186,65 @@ struct Tile {
     return PAIRED ? ((row >> 1) & 1) | (((row >> 3) & 3) << 1) : (row >> 1) & 7;
   }
 
-  // Rows [o0, o0 + ROWS) of O, r in [r0, r0 + kDepth) below r_end (zeros from there on).  A row past
-  // the last is some other row: its results are not stored.  base1: rows from SPLIT on.
+  // Rows [o0, o0 + ROWS) of O, r in [r0, r0 + kDepth) below r_end (zeros from there on) of R.  A row
+  // past the last is some other row: its results are not stored.  base1: rows from SPLIT on.
   template <int SPLIT>
-  static __device__ __forceinline__ void load(Chunk<T> (&c)[kChunks], const T* base, const T* base1,
-                                              int64_t ld, int64_t o0, int64_t O, int64_t r0, int64_t r_end) {
-    const bool whole = r0 + kDepth <= r_end && (RC || o0 + ROWS <= O);
+  static __device__ __forceinline__ void load(Chunk<T> (&c)[kChunks], const T* base, const T* base1, int64_t ld,
+                                              int64_t o0, int64_t O, int64_t r0, int64_t r_end, int64_t R) {
+    const bool deep = r0 + kDepth <= r_end;
+    const bool spare = (RC ? o0 + (SPLIT ? SPLIT : ROWS) + kSpareRows <= O : r0 + kDepth + kSpareRows <= R);
+    auto each = [&](auto kind) {
+      constexpr int KIND = decltype(kind)::value;  // 0: all there, 1: whole words, 2: element by element
+#pragma unroll
+      for (int s = 0; s < kChunks; s++) {
+        const int q = s * THREADS + threadIdx.x, row = q / kPerRow, col = q % kPerRow * 8;
+        if (RC) {
+          const bool second = SPLIT && row >= SPLIT;
+          int64_t o = o0 + (second ? row - SPLIT : row);
+          o = o < O ? o : O - 1;
+          const T* p = (second ? base1 : base) + o * ld;
+          if (KIND == 0) c[s] = load_whole(p + r0 + col);
+          else if (KIND == 1) c[s] = load_masked(p, r0 + col, r_end);
+          else c[s] = load_tail(p, r0 + col, 1, r_end);
+        } else {
+          if (KIND == 0) {
+            c[s] = load_whole(base + (r0 + row) * ld + o0 + col);
+          } else if (KIND == 1) {
+            c[s] = load_whole(base + (r0 + row) * ld + (o0 + col < O ? o0 + col : o0));
+          } else {
+            const bool in = r0 + row < r_end;
+            c[s] = load_tail(base + (in ? r0 + row : r_end - 1) * ld, o0 + col, 1, O);
+#pragma unroll
+            for (int k = 0; k < Operand<T>::kRaw; k++) c[s].w[k] = in ? c[s].w[k] : u32x4{0, 0, 0, 0};
+          }
+        }
+      }
+    };
+    if (deep && (RC || o0 + ROWS <= O)) each(Const<0>());
+    else if (spare && (RC || deep)) each(Const<1>());
+    else each(Const<2>());
+  }
+
+  // All there and every row and base a multiple of 16 bytes: straight into LDS, 1 KB per
+  // instruction, each lane fetching the chunk that belongs where it writes (16-bit types).
+  static __device__ __forceinline__ void direct(char* lds, const T* base, const T* base1, int split, int64_t ld,
+                                                int64_t o0, int64_t O, int64_t r0) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int s = 0; s < kChunks; s++) {
-      const int q = s * THREADS + threadIdx.x, row = q / kPerRow, col = q % kPerRow * 8;
+      const int q = s * THREADS + threadIdx.x, row = q / kPerRow, col = (q % kPerRow ^ swizzle(row)) * 8;
+      const T* p;
       if (RC) {
-        const bool second = SPLIT && row >= SPLIT;
-        int64_t o = o0 + (second ? row - SPLIT : row);
+        const bool second = split && row >= split;
+        int64_t o = o0 + (second ? row - split : row);
         o = o < O ? o : O - 1;
-        const T* p = (second ? base1 : base) + o * ld;
-        c[s] = whole ? load_whole(p + r0 + col) : load_tail(p, r0 + col, 1, r_end);
-      } else if (whole) {
-        c[s] = load_whole(base + (r0 + row) * ld + o0 + col);
+        p = (second ? base1 : base) + o * ld + r0 + col;
       } else {
-        const bool in = r0 + row < r_end;
-        c[s] = load_tail(base + (in ? r0 + row : r_end - 1) * ld, o0 + col, 1, O);
-#pragma unroll
-        for (int k = 0; k < Operand<T>::kRaw; k++) c[s].w[k] = in ? c[s].w[k] : u32x4{0, 0, 0, 0};
+        p = base + (r0 + row) * ld + o0 + col;
       }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                       (__attribute__((address_space(3))) void*)(lds + (s * THREADS + wave * 64) * 16),
+                                       16, 0, 0);
     }
   }
 
@@ -298,7 +353,6 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_
 }
 
 // f(integral constant of the activation): one branch for a whole epilogue.
-template <int V> struct Const { static constexpr int value = V; };
 template <int EPI, typename F>
 __device__ __forceinline__ void with_act(int act, F f) {
   if (EPI != EPI_FORWARD && EPI != EPI_DZ) return f(Const<GSR_ACT_NONE>());
@@ -343,8 +397,8 @@ __device__ __forceinline__ Place place(uint32_t tiles_i, uint32_t tiles_j, uint3
 
 // WI x WJ waves; a wave has BI / WI rows i and BJ / WJ rows j of the tile.  GATED: the tile's BJ
 // rows are BJ / 2 of the gate's weights and the same BJ / 2 of the up weights.
-template <typename T, bool RCA, bool RCB, int EPI, bool GATED, int BI, int WI, int BJ, int WJ>
-__global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, uint32_t tiles_i,
+template <typename T, bool RCA, bool RCB, int EPI, bool GATED, bool DIRECT, int BI, int WI, int BJ, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p, uint32_t tiles_i,
                                                                uint32_t tiles_j, uint32_t splits) {
   constexpr int NT = 64 * WI * WJ, kDepth = Operand<T>::kDepth, kPlanes = Operand<T>::kPlanes;
   constexpr int kBuffers = Operand<T>::kBuffers;
@@ -371,7 +425,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
   const uint32_t total = EPI == EPI_PLAIN ? steps * p.segments : steps;
 
   Chunk<T> ca[TA::kChunks], cb[TB::kChunks];
-  auto load = [&](uint32_t it) {
+  constexpr int kSplit = GATED ? BJ / 2 : 0;
+  // Where step `it` starts: f(A, B, r0).
+  auto at_step = [&](uint32_t it, auto f) {
     const T* a = (const T*)p.a;
     const T* b = (const T*)p.b[0];
     if (EPI == EPI_PLAIN && it >= steps) {  // the second segment
@@ -379,9 +435,13 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
       a += p.a_segment;
       b = (const T*)p.b[1];
     }
-    const int64_t r0 = r_begin + (int64_t)it * kDepth;
-    TA::template load<0>(ca, a, nullptr, lda, i0, p.I, r0, r_end);
-    TB::template load<GATED ? BJ / 2 : 0>(cb, b, (const T*)p.b[1], ldb, j0, p.J, r0, r_end);
+    f(a, b, r_begin + (int64_t)it * kDepth);
+  };
+  auto load = [&](uint32_t it) {
+    at_step(it, [&](const T* a, const T* b, int64_t r0) {
+      TA::template load<0>(ca, a, nullptr, lda, i0, p.I, r0, r_end, p.R);
+      TB::template load<kSplit>(cb, b, (const T*)p.b[1], ldb, j0, p.J, r0, r_end, p.R);
+    });
   };
   auto store = [&](int buffer) {
     char* s = lds + buffer * (TA::kBytes + TB::kBytes);
@@ -421,8 +481,31 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
     }
   };
 
-  load(0);
-  if constexpr (kBuffers == 2) {
+  if constexpr (DIRECT) {
+    // a step goes straight to LDS while the step before it is worked on
+    const bool columns = (RCA || i0 + BI <= p.I) && (RCB || j0 + kOut <= p.J);
+    auto stage = [&](uint32_t it, int buffer) {
+      at_step(it, [&](const T* a, const T* b, int64_t r0) {
+        if (columns && r0 + kDepth <= r_end) {
+          char* s = lds + buffer * (TA::kBytes + TB::kBytes);
+          TA::direct(s, a, nullptr, 0, lda, i0, p.I, r0);
+          TB::direct(s + TA::kBytes, b, (const T*)p.b[1], kSplit, ldb, j0, p.J, r0);
+        } else {
+          load(it);
+          store(buffer);
+        }
+      });
+    };
+    stage(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (uint32_t it = 0; it < total; it++) {
+      barrier();  // every wave's part of this step is there, and everyone has left the other buffer
+      if (it + 1 < total) stage(it + 1, (it + 1) & 1);
+      compute(it & 1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+  } else if constexpr (kBuffers == 2) {
+    load(0);
     store(0);
     for (uint32_t it = 0; it < total; it++) {
       __syncthreads();  // everyone has stored this step and left the other buffer
@@ -431,6 +514,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void product_kernel(ProductArgs p, ui
       if (it + 1 < total) store((it + 1) & 1);
     }
   } else {
+    load(0);
     for (uint32_t it = 0; it < total; it++) {
       if (it) __syncthreads();  // everyone has left the buffer
       store(0);
@@ -521,8 +605,16 @@ int launch_product(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   const int64_t ti = (p.I + BI - 1) / BI, tj = (p.J + kOut - 1) / kOut;
   if (ti > 0x7fffffff / tj || ti * tj > 0x7ffffff0 / splits) return 1;
   const int64_t total = ti * tj * splits, grid = (total + 7) / 8 * 8;
-  hipLaunchKernelGGL((product_kernel<T, RCA, RCB, EPI, GATED, BI, WI, BJ, WJ>), dim3((uint32_t)grid),
-                     dim3(64 * WI * WJ), 0, stream, p, (uint32_t)ti, (uint32_t)tj, (uint32_t)splits);
+  // straight to LDS where every 16-byte chunk is aligned
+  const uint64_t bits = (uint64_t)p.a | (uint64_t)p.b[0] | (uint64_t)p.b[1] |
+                        (uint64_t)((RCA ? p.a_i : p.a_r) | (RCB ? p.b_j : p.b_r) | p.a_segment) * sizeof(T);
+  auto go = [&](auto direct) {
+    hipLaunchKernelGGL((product_kernel<T, RCA, RCB, EPI, GATED, decltype(direct)::value, BI, WI, BJ, WJ>),
+                       dim3((uint32_t)grid), dim3(64 * WI * WJ), 0, stream, p, (uint32_t)ti, (uint32_t)tj,
+                       (uint32_t)splits);
+  };
+  if (sizeof(T) == 2 && bits % 16 == 0) go(Const<sizeof(T) == 2>());
+  else go(Const<0>());
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 

@@ -118,6 +118,7 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
   };
 
   fetch(0, 0);
+  const bool spare = i0 + 16 * NI + kSpareRows <= p.I;
   s16x8 a[NI][KS][kPlanes];
 #pragma unroll
   for (int u = 0; u < NI; u++) {
@@ -129,7 +130,7 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
       if (RCA) {
         const T* x = (const T*)p.a + i * p.a_i;
         if (kk * 32 + 32 <= K) c = load_whole(x + k);
-        else if (kk * 32 < K) c = load_tail(x, k, 1, K);
+        else if (kk * 32 < K) c = spare ? load_masked(x, k, K) : load_tail(x, k, 1, K);
       } else if (kk * 32 < K) {
         c = load_tail((const T*)p.a + i, k, p.a_r, K);
       }
