@@ -47,41 +47,55 @@ template <> __device__ __forceinline__ __hip_bfloat16 from_f<__hip_bfloat16>(flo
   return __float2bfloat16(v);
 }
 
-// The normal distribution's integral and exp(-z^2/2): Abramowitz & Stegun 7.1.26 (a rational
-// approximation of erf, absolute error below 1.5e-7, a float's own rounding next to 1), which
-// shares its exponential with the density that gelu's slope needs.
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float x = fabsf(z) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
-  e = __expf(-x * x);
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * p * t * e;  // 1 - cdf(|z|)
-  return z < 0.0f ? tail : 1.0f - tail;
+// gelu(z) = z cdf(z) = max(z, 0) - |z| T(|z|), T(a) = cdf(-a), the normal distribution's tail.
+// log2 T is nearly a parabola: a weighted minimax polynomial of degree 8 on [0, 8] (fitted to
+// T itself) gives |z| T to 5e-8 with one exponential and no division.  Beyond 8 the tail is 0 in 32
+// bits.  NaN and -inf give NaN, as 0.5 z (1 + erf(z / sqrt 2)) does.
+__device__ __forceinline__ float relu_exact(float z) { return fmaf(0.5f, z, 0.5f * fabsf(z)); }
+__device__ __forceinline__ float gelu_value(float z) {
+  const float a = fminf(fabsf(z), 8.0f);
+  float p = fmaf(-1.9919228e-06f, a, 2.9272256e-05f);
+  p = fmaf(p, a, -1.380893e-04f);
+  p = fmaf(p, a, -2.5343438e-04f);
+  p = fmaf(p, a, 7.2163874e-03f);
+  p = fmaf(p, a, -5.2603047e-02f);
+  p = fmaf(p, a, -4.5917222e-01f);
+  p = fmaf(p, a, -1.1511097f);
+  p = fmaf(p, a, -0.9999999f);
+  return fmaf(-a, __builtin_amdgcn_exp2f(p), relu_exact(z));
+}
+// gelu'(z) = 1/2 + sign(z) (1/2 - h(|z|)), h(a) = T(a) - a density(a) = exp(-a^2/2) Q(a): the
+// exponential has the steep part, Q is a minimax polynomial of degree 10 on [0, 6] (h to 1.7e-7).
+// The value shares both: T(a) = exp(-a^2/2) (Q(a) + a / sqrt(2 pi)).
+__device__ __forceinline__ float gelu_both(float z, float& value) {
+  const float a = fminf(fabsf(z), 6.0f);
+  const float e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);
+  float q = fmaf(1.2712853e-06f, a, -2.8994787e-05f);
+  q = fmaf(q, a, 2.951621e-04f);
+  q = fmaf(q, a, -1.8013967e-03f);
+  q = fmaf(q, a, 7.5418255e-03f);
+  q = fmaf(q, a, -2.3762807e-02f);
+  q = fmaf(q, a, 6.0701676e-02f);
+  q = fmaf(q, a, -1.3230555e-01f);
+  q = fmaf(q, a, 2.4986956e-01f);
+  q = fmaf(q, a, -7.9787475e-01f);
+  q = fmaf(q, a, 4.9999988e-01f);
+  value = fmaf(-a, e * fmaf(a, 0.39894228f, q), relu_exact(z));
+  return fmaf(z, 0.0f, 0.5f) + copysignf(fmaf(-e, q, 0.5f), z);  // z * 0: NaN stays NaN
 }
 
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == GSR_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-  if constexpr (ACT == GSR_ACT_GELU) {
-    float e;
-    return z * normal_cdf(z, e);
-  }
+  if constexpr (ACT == GSR_ACT_GELU) return gelu_value(z);
   if constexpr (ACT == GSR_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
   return z;
 }
 
-// The activation's value and slope at z.
+// The activation's slope at z, and its value.
 template <int ACT>
 __device__ __forceinline__ float act_both(float z, float& value) {
-  if constexpr (ACT == GSR_ACT_GELU) {
-    float e;
-    const float c = normal_cdf(z, e);
-    value = z * c;
-    return fmaf(z * 0.39894228040143268f, e, c);
-  }
+  if constexpr (ACT == GSR_ACT_GELU) return gelu_both(z, value);
   if constexpr (ACT == GSR_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
     value = z * s;

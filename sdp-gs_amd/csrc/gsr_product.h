@@ -108,17 +108,56 @@ __device__ __forceinline__ Chunk<T> load_masked(const T* row, int64_t k, int64_t
 }
 constexpr int kSpareRows = 8;  // with so many rows after it, a row may be read 7 elements too far
 
-// 16 bytes of a row of n elements from element k on; those past its end repeat its last.
-template <typename T>
-__device__ __forceinline__ u32x4 load_tail_words(const T* row, int64_t k, int64_t n) {
-  u32x4 w = {0, 0, 0, 0};
+// N words moved down by `off` elements (0..7), zeros from above.
+template <typename T, int N>
+__device__ __forceinline__ void shift_down(uint32_t (&w)[N], int off) {
+  const int words = sizeof(T) == 4 ? off : off >> 1;
 #pragma unroll
-  for (int e = 0; e < (int)(16 / sizeof(T)); e++) {
-    const int64_t at = k + e < n ? k + e : n - 1;
-    if constexpr (sizeof(T) == 4) w[e] = ((const uint32_t*)row)[at];
-    else w[e >> 1] |= (uint32_t)((const uint16_t*)row)[at] << (16 * (e & 1));
+  for (int bit = 4; bit; bit >>= 1) {
+    if (bit >= N) continue;
+#pragma unroll
+    for (int e = 0; e < N; e++) w[e] = words & bit ? (e + bit < N ? w[e + bit] : 0u) : w[e];
   }
-  return w;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const uint32_t next = e + 1 < N ? w[e + 1] : 0u;
+      w[e] = off & 1 ? w[e] >> 16 | next << 16 : w[e];
+    }
+  }
+}
+// Elements k..k+7 of a row of n; those past its end are zero.  One read of whole words and no
+// branch: at the end of the tensor (`end`: past its last element, at least 8 after its first) an
+// earlier place is read and moved down.
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_row_end(const T* row, int64_t k, int64_t n, const T* end) {
+  constexpr int N = 4 * Operand<T>::kRaw;
+  const T* p = row + (k < n ? k : 0);
+  const int off = p + 8 > end ? (int)(p + 8 - end) : 0;
+  const Chunk<T> c = load_whole(p - off);
+  uint32_t w[N];
+#pragma unroll
+  for (int e = 0; e < N; e++) w[e] = c.w[e >> 2][e & 3];
+  shift_down<T, N>(w, off);
+  const int64_t left = n - k;
+  Chunk<T> r;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    if constexpr (sizeof(T) == 4) r.w[e >> 2][e & 3] = e < left ? w[e] : 0u;
+    else r.w[0][e] = w[e] & (2 * e + 1 < left ? ~0u : 2 * e < left ? 0xffffu : 0u);
+  }
+  return r;
+}
+// The same for the 16 bytes at element k, anything in the place of those past the row's end.
+template <typename T>
+__device__ __forceinline__ u32x4 load_words_end(const T* row, int64_t k, int64_t n, const T* end) {
+  constexpr int RUN = 16 / sizeof(T);
+  const T* p = row + (k < n ? k : 0);
+  const int off = p + RUN > end ? (int)(p + RUN - end) : 0;
+  const u32x4 c = ((const Bytes16*)(p - off))->v;
+  uint32_t w[4] = {c[0], c[1], c[2], c[3]};
+  shift_down<T, 4>(w, off);
+  return u32x4{w[0], w[1], w[2], w[3]};
 }
 
 // Which parts are multiplied: smallest products first.
@@ -333,14 +372,17 @@ __device__ __forceinline__ void store_run(T* p, const float (&v)[RUN], int64_t n
 }
 
 // The epilogue of RUN results v (and w, the up half) of row i at columns j..; n of them exist.
-template <typename T, int EPI, bool GATED, int ACT, int RUN>
+// EXTRA: with ex, the residual or the incoming gradient.
+template <typename T, int EPI, bool GATED, bool EXTRA, int ACT, int RUN>
 __device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_t j, int64_t n,
                                          float (&v)[RUN], float (&w)[RUN], const float (&ex)[RUN]) {
   T* out = (T*)p.out + i * p.out_row + j;
 #pragma unroll
   for (int k = 0; k < RUN; k++) {
     if (EPI == EPI_FORWARD) {
-      v[k] = GATED ? act_value<ACT>(v[k]) * w[k] : act_value<ACT>(v[k]) + ex[k];
+      v[k] = act_value<ACT>(v[k]);
+      if (GATED) v[k] *= w[k];
+      if (EXTRA) v[k] += ex[k];
     } else if (EPI == EPI_DZ) {
       float a;
       const float s = act_both<ACT>(v[k], a);
@@ -592,7 +634,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
           store_run<float, RUN>(p.part + ((int64_t)at.split * p.I + i) * p.J + j, v, n);
         } else {
           if (EPI != EPI_PLAIN && p.extra) load_run<T, RUN>(ex, (const T*)p.extra + i * p.extra_row + j, n);
-          epilogue<T, EPI, GATED, decltype(act)::value, RUN>(p, i, j, n, v, w, ex);
+          epilogue<T, EPI, GATED, true, decltype(act)::value, RUN>(p, i, j, n, v, w, ex);
         }
       }
     }

@@ -3,23 +3,24 @@
 //
 // At these widths a tile of C has only a few steps along K, so a tiled kernel spends its time
 // filling and draining pipelines.  Here a wave loads all of its 16 NI rows at once, straight into
-// the matrix instruction's operand layout (every byte of x is read once, and all of a workgroup's
-// reads are in flight together).  The weights are first written out once as the images that LDS is
-// to hold (16-bit parts, padded with zeros to whole tiles, rows in reading order): a tile's image
-// goes to LDS by direct loads without passing registers or needing bounds, two tiles ahead, so that
-// neither it nor the stores of finished results are waited for.
+// the matrix instruction's operand layout (every byte of x is read once).  The weights are first written out once as the images that LDS is to hold (16-bit parts,
+// padded with zeros to whole tiles, rows in reading order, biases among them): a tile's image goes
+// to LDS by direct loads without passing registers or needing bounds, the next one while this one
+// is worked on, and a tile's results leave as soon as they are there.
 #pragma once
 #include "gsr_rows.h"
 
 namespace gsr {
 
-// kRows rows of weights in a tile, kWaves waves of 16 kNI rows of x, for up to 32 KS inputs: three
-// tiles of two or three workgroups fit the LDS of a CU (of one with twice the waves, gated: a tile
-// has the rows of both halves).
+// kRows rows of weights in a tile (128 bytes of a result's row; gated, 64 of each half's), kWaves
+// waves of 16 kNI rows of x, for up to 32 KS inputs; kGroups workgroups to a CU, as many as its
+// registers and LDS hold.
 template <typename T, int KS, bool GATED> struct Strip {
-  static constexpr int kNI = sizeof(T) == 4 && KS > 4 ? 1 : 2;  // three parts of x fill the registers
-  static constexpr int kWaves = GATED && sizeof(T) == 4 && KS > 6 ? 8 : 4;
-  static constexpr int kRows = sizeof(T) == 4 ? (KS > 6 && !GATED ? 16 : 32) : 64;
+  static constexpr bool kSplit = sizeof(T) == 4;
+  static constexpr int kNI = kSplit && KS > 4 ? 1 : 2;  // three parts of x fill the registers
+  static constexpr int kWaves = kSplit && KS > 6 ? 8 : 4;
+  static constexpr int kRows = kSplit ? 32 : 64;
+  static constexpr int kGroups = kSplit && KS > 6 ? 1 : kSplit || KS > 2 ? 2 : 3;
   static constexpr int kOut = GATED ? kRows / 2 : kRows;  // outputs of a tile
   // Bytes of a row: the 32 of padding turn it by two of the 16 bank groups, so that the lanes that
   // a 16-byte read takes together (0-3, 12-15, 20-23, 24-27 and so on) hit different ones.  The
@@ -61,7 +62,8 @@ __global__ __launch_bounds__(256) void image_kernel(ProductArgs p, char* images,
   put_chunk<T>(image + place * S::kRow + at * 16, S::kPlane, c);
 }
 
-template <typename T, bool RCA, int EPI, bool GATED, int KS>
+// EXTRA: there is a residual (forward).
+template <typename T, bool RCA, int EPI, bool GATED, bool EXTRA, int KS>
 __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_kernel(
     ProductArgs p, const char* images, uint32_t strips, uint32_t parts, uint32_t part_tiles) {
   using S = Strip<T, KS, GATED>;
@@ -71,27 +73,19 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
   static_assert(kRuns >= 1 && NJ >= 1, "");
   __shared__ __attribute__((aligned(1024))) char lds[2 * S::kImage];
 
-  const uint32_t each = gridDim.x >> 3, id = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
-  if (id >= strips * parts) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int m = lane & 15, q = lane >> 4;
   const int K = (int)p.R;
+  const uint32_t each = gridDim.x >> 3, id = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  if (id >= strips * parts) return;
   const int64_t i0 = ((int64_t)(id / parts) * kWaves + wave) * (16 * NI);
-  const uint32_t tile0 = id % parts * part_tiles, all = (uint32_t)((p.J + kOut - 1) / kOut);
-  const uint32_t tile1 = tile0 + part_tiles < all ? tile0 + part_tiles : all;
-  if (tile0 >= tile1) return;
-  // Workgroups start at different tiles: rows of a power of two would otherwise have all of them
-  // write to the same few memory channels at a time.
-  const uint32_t count = tile1 - tile0, turn = id / parts % count;
-  auto tile_at = [&](uint32_t t) {
-    t = t < count ? t : count - 1;
-    return tile0 + (t + turn < count ? t + turn : t + turn - count);
-  };
+  const uint32_t tiles = (uint32_t)((p.J + kOut - 1) / kOut), tile0 = id % parts * part_tiles;
+  const uint32_t tile1 = tile0 + part_tiles < tiles ? tile0 + part_tiles : tiles;
 
   // An image into LDS, 1 KB per instruction; every wave issues as many (the last KB more than once).
   constexpr int kFetches = (S::kImage / 1024 + kWaves - 1) / kWaves;
-  auto fetch = [&](uint32_t t, uint32_t buffer) {
-    const char* src = images + (size_t)tile_at(t) * S::kImage + lane * 16;
+  auto fetch = [&](uint32_t tile, int buffer) {
+    const char* src = images + (size_t)tile * S::kImage + lane * 16;
     char* to = lds + buffer * S::kImage;
 #pragma unroll
     for (int u = 0; u < kFetches; u++) {
@@ -105,20 +99,20 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
     return i < p.I ? i : p.I - 1;
   };
   auto column_of = [&](int s) { return kPaired ? 32 * s + 8 * q : 16 * s + 4 * q; };
-  auto load_extra = [&](u32x4 (&ex)[NI][kRuns], uint32_t t) {
-    const int64_t j0 = (int64_t)tile_at(t) * kOut;
+  auto load_extra = [&](u32x4 (&ex)[NI][kRuns], uint32_t tile) {
+    const int64_t j0 = (int64_t)tile * kOut;
     const bool whole = j0 + kOut <= p.J;
 #pragma unroll
     for (int u = 0; u < NI; u++)
 #pragma unroll
       for (int s = 0; s < kRuns; s++) {
         const T* e = (const T*)p.extra + row_of(u) * p.extra_row;
-        ex[u][s] = whole ? ((const Bytes16*)(e + j0 + column_of(s)))->v : load_tail_words(e, j0 + column_of(s), p.J);
+        ex[u][s] = whole ? ((const Bytes16*)(e + j0 + column_of(s)))->v
+                         : load_words_end(e, j0 + column_of(s), p.J, (const T*)p.extra + (p.I - 1) * p.extra_row + p.J);
       }
   };
-
-  fetch(0, 0);
-  const bool spare = i0 + 16 * NI + kSpareRows <= p.I;
+  const T* const x_end = (const T*)p.a + (p.I - 1) * p.a_i + K;
+  fetch(tile0, 0);
   s16x8 a[NI][KS][kPlanes];
 #pragma unroll
   for (int u = 0; u < NI; u++) {
@@ -130,7 +124,7 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
       if (RCA) {
         const T* x = (const T*)p.a + i * p.a_i;
         if (kk * 32 + 32 <= K) c = load_whole(x + k);
-        else if (kk * 32 < K) c = spare ? load_masked(x, k, K) : load_tail(x, k, 1, K);
+        else if (kk * 32 < K) c = load_row_end(x, k, K, x_end);
       } else if (kk * 32 < K) {
         c = load_tail((const T*)p.a + i, k, p.a_r, K);
       }
@@ -138,110 +132,124 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
     }
   }
   u32x4 ex[NI][kRuns] = {}, ex_next[NI][kRuns] = {};
-  if (p.extra) load_extra(ex, 0);
+  if (EXTRA) load_extra(ex, tile0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  const bool rows_in = i0 + 16 * NI <= p.I;
+  int buffer = 0;
 
-  for (uint32_t step = 0, buffer = 0; step < count; step++) {
-    // every wave's part of this image is in LDS, and everyone has left the image before it
-    barrier();
-    fetch(step + 1, buffer ^ 1);
-    if (p.extra) load_extra(ex_next, step + 1);
-    const int64_t j0 = (int64_t)tile_at(step) * kOut;
-    const char* image = lds + buffer * S::kImage;
-    f32x4 acc[NI][NJ] = {};
-    // the operands of kAhead reads are on their way while the products of the one before are formed
-    constexpr int kReads = KS * NJ, kAhead = kReads * kPlanes < 8 ? kReads : 8 / kPlanes;
-    s16x8 b[kAhead][kPlanes];
-    auto read = [&](int n) {
-      const int kk = n / NJ, t = n % NJ;
+  with_act<EPI>(p.act, [&](auto act) {
+      // One tile.  FULL: it lies within C, so its epilogue has no branch and stores kStores times.
+      auto step = [&](auto full, uint32_t tile) {
+        constexpr bool FULL = decltype(full)::value;
+        // every wave's part of this image is in LDS, and everyone has left the image before it
+        barrier();
+        const uint32_t next = tile + 1 < tile1 ? tile + 1 : tile;
+        fetch(next, buffer ^ 1);
+        if (EXTRA) load_extra(ex_next, next);
+        const int64_t j0 = (int64_t)tile * kOut;
+        const char* image = lds + buffer * S::kImage;
+        // the biases (8 of them to a row's padding) are what the sums start from
+        f32x4 acc[NI][NJ];
 #pragma unroll
-      for (int z = 0; z < kPlanes; z++)
-        b[n % kAhead][z] = *(const s16x8*)(image + z * S::kPlane + (16 * t + m) * S::kRow + (kk * 4 + q) * 16);
-    };
+        for (int t = 0; t < NJ; t++) {
+          const int row = kPaired ? 32 * (t >> 1) + 8 * q + 4 * (t & 1) : 16 * t + 4 * q;
+          f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (EPI != EPI_PLAIN) bias = *(const f32x4*)(image + row / 8 * S::kRow + KS * 64 + row % 8 * 4);
 #pragma unroll
-    for (int n = 0; n < kAhead; n++) read(n);
-#pragma unroll
-    for (int n = 0; n < kReads; n++) {
-      const int kk = n / NJ, t = n % NJ;
-#pragma unroll
-      for (int k = 0; k < Parts<kPlanes>::kProducts; k++)
-#pragma unroll
-        for (int u = 0; u < NI; u++)
-          acc[u][t] = mfma<T>(b[n % kAhead][Parts<kPlanes>::kB[k]], a[u][kk][Parts<kPlanes>::kA[k]], acc[u][t]);
-      if (n + kAhead < kReads) read(n + kAhead);
-      __builtin_amdgcn_sched_barrier(0);  // keeps this order
-    }
-    if constexpr (sizeof(T) == 4) {
-      float odd = 0.0f;  // stays 0 while every result is finite
-#pragma unroll
-      for (int u = 0; u < NI; u++)
-#pragma unroll
-        for (int t = 0; t < NJ; t++)
-#pragma unroll
-          for (int v = 0; v < 4; v++) odd = fmaf(acc[u][t][v], 0.0f, odd);
-      if (odd != 0.0f) {
-#pragma unroll
-        for (int u = 0; u < NI; u++)
-#pragma unroll
-          for (int t = 0; t < NJ; t++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) {
-              const int row = t * 16 + 4 * q + v;
-              const bool second = GATED && row >= kOut;
-              const int64_t i = i0 + u * 16 + m, j = j0 + (second ? row - kOut : row);
-              if (i < p.I && j < p.J && !(fabsf(acc[u][t][v]) <= 3.4e38f))
-                acc[u][t][v] = exact_sum((const float*)p.a, p.a_i, p.a_r, (const float*)p.b[second ? 1 : 0],
-                                         nullptr, p.b_j, p.b_r, 1, 0, i, j, 0, K);
-            }
-      }
-    }
-    const bool whole = rows_in && j0 + kOut <= p.J;
-    auto finish = [&](auto act, auto full) {
-      constexpr bool FULL = decltype(full)::value;
-#pragma unroll
-      for (int s = 0; s < kRuns; s++) {
-        const int64_t j = j0 + column_of(s), n = FULL ? RUN : p.J - j;
-        if (!FULL && n <= 0) continue;
-        float bias[RUN] = {}, bias1[RUN] = {};
-        auto load_bias = [&](float (&v)[RUN], int row) {
-          const f32x4* w = (const f32x4*)(image + row / 8 * S::kRow + KS * 64 + row % 8 * 4);
-#pragma unroll
-          for (int k = 0; k < RUN; k++) v[k] = w[k / 4][k % 4];
-        };
-        if (EPI != EPI_PLAIN) load_bias(bias, column_of(s));
-        if (EPI != EPI_PLAIN && GATED) load_bias(bias1, kOut + column_of(s));
-#pragma unroll
-        for (int u = 0; u < NI; u++) {
-          const int64_t i = i0 + u * 16 + m;
-          if (!FULL && i >= p.I) continue;
-          float v[RUN], w[RUN], e[RUN];
-          widen<T, RUN>(e, ex[u][s]);
-#pragma unroll
-          for (int k = 0; k < RUN; k++) {
-            v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4] + bias[k];
-            if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4] + bias1[k];
-          }
-          epilogue<T, EPI, GATED, decltype(act)::value, RUN>(p, i, j, n, v, w, e);
+          for (int u = 0; u < NI; u++) acc[u][t] = bias;
         }
-      }
-    };
-    with_act<EPI>(p.act, [&](auto act) {
-      if (whole) finish(act, Const<1>());
-      else finish(act, Const<0>());
-    });
-    // This wave's part of the next image has to be there.  It was asked for before the stores of
-    // this tile, which may go on: a whole tile has kStores of them.
-    constexpr int kStores = NI * kRuns * (EPI == EPI_DZ && GATED ? 2 : 1);
-    if (whole) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // the operands of kQueue reads are on their way while the products of the one before are formed
+        constexpr int kReads = KS * NJ, kQueue = kReads * kPlanes < 8 ? kReads : 8 / kPlanes;
+        s16x8 b[kQueue][kPlanes];
+        auto read = [&](int n) {
+          const int kk = n / NJ, t = n % NJ;
 #pragma unroll
-    for (int u = 0; u < NI; u++)
+          for (int z = 0; z < kPlanes; z++)
+            b[n % kQueue][z] = *(const s16x8*)(image + z * S::kPlane + (16 * t + m) * S::kRow + (kk * 4 + q) * 16);
+        };
 #pragma unroll
-      for (int s = 0; s < kRuns; s++) ex[u][s] = ex_next[u][s];
-    buffer ^= 1;
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing arrives in LDS that is another's
+        for (int n = 0; n < kQueue; n++) read(n);
+        // Two workgroups that are both at their products would stay in step and leave memory idle
+        // in between: one of the two gives way to the other.
+        if (S::kGroups == 2) {
+          if (blockIdx.x >> 8 & 1) __builtin_amdgcn_s_setprio(1);
+          else __builtin_amdgcn_s_setprio(0);
+        }
+#pragma unroll
+        for (int n = 0; n < kReads; n++) {
+          const int kk = n / NJ, t = n % NJ;
+#pragma unroll
+          for (int k = 0; k < Parts<kPlanes>::kProducts; k++)
+#pragma unroll
+            for (int u = 0; u < NI; u++)
+              acc[u][t] = mfma<T>(b[n % kQueue][Parts<kPlanes>::kB[k]], a[u][kk][Parts<kPlanes>::kA[k]], acc[u][t]);
+          if (n + kQueue < kReads) read(n + kQueue);
+          __builtin_amdgcn_sched_barrier(0);  // keeps this order
+        }
+        if (S::kGroups == 2) __builtin_amdgcn_s_setprio(3);
+        if constexpr (sizeof(T) == 4) {
+          float odd = 0.0f;  // stays 0 while every result is finite
+#pragma unroll
+          for (int u = 0; u < NI; u++)
+#pragma unroll
+            for (int t = 0; t < NJ; t++)
+#pragma unroll
+              for (int v = 0; v < 4; v++) odd = fmaf(acc[u][t][v], 0.0f, odd);
+          if (odd != 0.0f) {
+#pragma unroll
+            for (int u = 0; u < NI; u++)
+#pragma unroll
+              for (int t = 0; t < NJ; t++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                  const int row = t * 16 + 4 * q + v;
+                  const bool second = GATED && row >= kOut;
+                  const int64_t i = i0 + u * 16 + m, j = j0 + (second ? row - kOut : row);
+                  if (i >= p.I || j >= p.J || fabsf(acc[u][t][v]) <= 3.4e38f) continue;
+                  const float* bias = (const float*)p.bias[second ? 1 : 0];
+                  acc[u][t][v] = exact_sum((const float*)p.a, p.a_i, p.a_r, (const float*)p.b[second ? 1 : 0],
+                                           nullptr, p.b_j, p.b_r, 1, 0, i, j, 0, K) +
+                                 (EPI != EPI_PLAIN && bias ? bias[j] : 0.0f);
+                }
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < kRuns; s++) {
+          const int64_t j = j0 + column_of(s), n = FULL ? RUN : p.J - j;
+          if (!FULL && n <= 0) continue;
+#pragma unroll
+          for (int u = 0; u < NI; u++) {
+            const int64_t i = i0 + u * 16 + m;
+            if (!FULL && i >= p.I) continue;
+            float v[RUN], w[RUN], e[RUN];
+            widen<T, RUN>(e, ex[u][s]);
+#pragma unroll
+            for (int k = 0; k < RUN; k++) {
+              v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4];
+              if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4];
+            }
+            epilogue<T, EPI, GATED, EXTRA, decltype(act)::value, RUN>(p, i, j, n, v, w, e);
+          }
+        }
+        // This wave's part of the next image has to be there.  It was asked for before the stores of
+        // this tile, which may go on.
+        constexpr int kStores = NI * kRuns * (EPI == EPI_DZ && GATED ? 2 : 1);
+        if (FULL) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (EXTRA) {
+#pragma unroll
+          for (int u = 0; u < NI; u++)
+#pragma unroll
+            for (int s = 0; s < kRuns; s++) ex[u][s] = ex_next[u][s];
+        }
+        buffer ^= 1;
+      };
+      // the tiles that lie within C, then the last ones of a ragged C
+      const uint32_t fit = i0 + 16 * NI <= p.I ? (uint32_t)(p.J / kOut) : 0;
+      uint32_t tile = tile0;
+      for (; tile < tile1 && tile < fit; tile++) step(Const<1>(), tile);
+      for (; tile < tile1; tile++) step(Const<0>(), tile);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing arrives in LDS that is another's
+  });
 }
 
 template <typename T, bool GATED, int KS>
@@ -255,17 +263,23 @@ int launch_strip(const ProductArgs& p, char* scratch, hipStream_t stream) {
   using S = Strip<T, KS, GATED>;
   constexpr int kOut = S::kOut, kBlock = S::kWaves * 16 * S::kNI;
   const int64_t strips = (p.I + kBlock - 1) / kBlock, tiles = (p.J + kOut - 1) / kOut;
-  const int64_t chunks = tiles * S::kRows * KS * 4;
-  // too few strips to give every CU two workgroups: several workgroups share one's outputs
-  int64_t parts = strips >= 512 ? 1 : (512 + strips - 1) / strips;
+  const int64_t chunks = tiles * S::kRows * KS * 4, groups = 256 * S::kGroups;
+  // fewer strips than workgroups: several share one's outputs
+  int64_t parts = strips >= groups ? 1 : (groups + strips - 1) / strips;
   if (parts > tiles) parts = tiles;
   const int64_t part_tiles = (tiles + parts - 1) / parts;
-  if (strips > 0x7ffffff0 / parts || chunks > 0x7fffffff) return 1;
+  parts = (tiles + part_tiles - 1) / part_tiles;
+  const int64_t items = strips * parts;
+  if (items > 0x7ffffff0 || chunks > 0x7fffffff) return 1;
   hipLaunchKernelGGL((image_kernel<T, GATED, KS>), dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, stream, p,
                      scratch, (uint32_t)chunks);
-  hipLaunchKernelGGL((strip_kernel<T, RCA, EPI, GATED, KS>), dim3((uint32_t)((strips * parts + 7) / 8 * 8)),
-                     dim3(64 * S::kWaves), 0, stream, p, (const char*)scratch, (uint32_t)strips, (uint32_t)parts,
-                     (uint32_t)part_tiles);
+  auto go = [&](auto extra) {
+    hipLaunchKernelGGL((strip_kernel<T, RCA, EPI, GATED, decltype(extra)::value, KS>),
+                       dim3((uint32_t)((items + 7) / 8 * 8)), dim3(64 * S::kWaves), 0, stream, p,
+                       (const char*)scratch, (uint32_t)strips, (uint32_t)parts, (uint32_t)part_tiles);
+  };
+  if (EPI == EPI_DZ || (EPI == EPI_FORWARD && !GATED && p.extra)) go(Const<EPI != EPI_PLAIN && !(EPI == EPI_FORWARD && GATED)>());
+  else go(Const<EPI == EPI_DZ>());
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
