@@ -12,8 +12,8 @@
  *   w, residual, y, dy, gradients: rows contiguous, any row stride >= the row's length
  * M = 0 is a no-op (weight gradients are set to zero); K and N are at least 1.
  * Every launch goes to `stream` on the current device.  scratch: device memory of the size the
- * matching *_scratch_bytes function gives, 256-byte aligned, untouched by others until the call's
- * work is done; it holds nothing between calls.  Results do not depend on timing (no atomics).
+ * matching *_scratch_bytes function gives (NULL for 0), 256-byte aligned, untouched by others until
+ * the call's work is done; it holds nothing between calls.  Results do not depend on timing (no atomics).
  * Returns 0, 1 on invalid arguments, 2 on a launch error.
  */
 #ifndef GSR_LINEAR_H

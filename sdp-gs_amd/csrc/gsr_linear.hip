@@ -5,18 +5,37 @@ namespace {
 
 using namespace gsr;
 
-// out[e] = sum over the splits of part[s][e], in a fixed order; the row sums follow the products.
+// out[e] = sum over the splits of part[s][e] in a fixed order; the row sums follow the products.
+// 64 outputs to a workgroup, the splits shared by its four waves (a wave of few outputs alone would
+// wait for one split after the other: 33 us for 128 splits of 203 x 161, against 8).
 template <typename T>
 __global__ __launch_bounds__(256) void reduce_kernel(const float* part, const float* part_sum,
                                                      int splits, int64_t n, int64_t n_sum, T* dw,
                                                      T* db) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const bool first = e < n;
-  if (!first && e - n >= n_sum) return;
-  const float* src = first ? part + e : part_sum + (e - n);
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t e = (int64_t)blockIdx.x * 64 + lane;
+  const bool first = e < n, in = first || e - n < n_sum;
+  const float* src = first ? part + e : part_sum + (in ? e - n : 0);
   const int64_t step = first ? n : n_sum;
+  const int each = (splits + 3) / 4, begin = wave * each;
+  const int end = begin + each < splits ? begin + each : splits;
   float v = 0.0f;
-  for (int s = 0; s < splits; s++) v += src[s * step];
+  if (in) {
+    int s = begin;
+    for (; s + 8 <= end; s += 8) {
+      float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) w[k] = src[(s + k) * step];
+#pragma unroll
+      for (int k = 0; k < 8; k++) v += w[k];
+    }
+    for (; s < end; s++) v += src[s * step];
+  }
+  sums[wave][lane] = v;
+  __syncthreads();
+  if (wave || !in) return;
+  v = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
   if (first) dw[e] = from_f<T>(v);
   else db[e - n] = from_f<T>(v);
 }
@@ -71,7 +90,7 @@ int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64
   p.part_sum = db ? p.part + splits * I * K : nullptr;
   if (int rc = product_dw<T>(p, splits, stream)) return rc;
   const int64_t n = dw ? I * K : 0, n_sum = db ? I : 0;
-  hipLaunchKernelGGL(reduce_kernel<T>, dim3((uint32_t)((n + n_sum + 255) / 256)), dim3(256), 0, stream,
+  hipLaunchKernelGGL(reduce_kernel<T>, dim3((uint32_t)((n + n_sum + 63) / 64)), dim3(256), 0, stream,
                      p.part, p.part_sum, (int)splits, n, n_sum, (T*)dw, (T*)db);
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
@@ -176,7 +195,7 @@ int forward(int dtype, const ProductArgs& p, bool gated, void* scratch, void* st
 size_t forward_bytes(int dtype, int64_t M, int64_t K, int64_t N, bool gated) {
   return with_type(dtype, [&](auto t) {
     return product_scratch<typename Pointee<decltype(t)>::type>(M, N, K, gated);
-  }) + 256;
+  });
 }
 
 }  // namespace
@@ -191,7 +210,8 @@ extern "C" int gsr_linear(int dtype, int64_t M, int64_t K, int64_t N, const void
                           int64_t y_row, void* scratch, void* stream) {
   if (!sizes_ok(dtype, M, K, N, act) || !x_ok(M, K, x_row, x_col) || w_row < K) return 1;
   if (M == 0) return 0;
-  if (!x || !w || !y || !scratch || y_row < N || (residual && residual_row < N && M > 1)) return 1;
+  if (!x || !w || !y || y_row < N || (residual && residual_row < N && M > 1)) return 1;
+  if (!scratch && forward_bytes(dtype, M, K, N, false)) return 1;
   ProductArgs p = forward_args(M, K, N, x, x_row, x_col, w, nullptr, w_row, bias, nullptr, act);
   p.extra = residual; p.extra_row = residual_row;
   p.out = y; p.out_row = y_row;
@@ -229,7 +249,8 @@ extern "C" int gsr_gated(int dtype, int64_t M, int64_t K, int64_t N, const void*
                          const void* bu, int act, void* h, int64_t h_row, void* scratch, void* stream) {
   if (!sizes_ok(dtype, M, K, N, act) || !x_ok(M, K, x_row, 1) || w_row < K) return 1;
   if (M == 0) return 0;
-  if (!x || !wg || !wu || !h || !scratch || h_row < N) return 1;
+  if (!x || !wg || !wu || !h || h_row < N) return 1;
+  if (!scratch && forward_bytes(dtype, M, K, N, true)) return 1;
   ProductArgs p = forward_args(M, K, N, x, x_row, 1, wg, wu, w_row, bg, bu, act);
   p.out = h; p.out_row = h_row;
   return forward(dtype, p, true, scratch, stream);

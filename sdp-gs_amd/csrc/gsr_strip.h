@@ -30,36 +30,31 @@ template <typename T, int KS, bool GATED> struct Strip {
   static constexpr int kImage = (kPlane * Operand<T>::kPlanes + 1023) / 1024 * 1024;
 };
 
-// One thread per 8 weights: tile, row, chunk.
+// Chunk `at` (8 weights) of row `row` of a tile's image; the first chunk brings the row's bias.
 template <typename T, bool GATED, int KS>
-__global__ __launch_bounds__(256) void image_kernel(ProductArgs p, char* images, uint32_t chunks) {
+__device__ __forceinline__ void image_chunk(const ProductArgs& p, uint32_t tile, int row, int at, char* image) {
   using S = Strip<T, KS, GATED>;
-  constexpr int LR = S::kRows, kOut = S::kOut;
-  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
-  if (id >= chunks) return;
-  const int at = id % (KS * 4), row = id / (KS * 4) % LR;
-  const uint32_t tile = id / (KS * 4 * LR);
-  const bool second = GATED && row >= kOut;
-  const int64_t j = (int64_t)tile * kOut + (second ? row - kOut : row);
-  const T* w = (const T*)p.b[second ? 1 : 0] + j * p.b_j;
-  char* image = images + (size_t)tile * S::kImage;
+  const bool second = GATED && row >= S::kOut;
+  const int64_t j = (int64_t)tile * S::kOut + (second ? row - S::kOut : row);
+  const bool in = j < p.J;
+  Chunk<T> c = load_tail((const T*)p.b[second ? 1 : 0] + (in ? j : 0) * p.b_j, at * 8, p.b_r, p.R);
+#pragma unroll
+  for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = in ? c.w[k] : u32x4{0, 0, 0, 0};
   if (at == 0) {
     const T* bias = (const T*)p.bias[second ? 1 : 0];
-    ((float*)(image + row / 8 * S::kRow + KS * 64))[row % 8] = bias && j < p.J ? to_f(bias[j]) : 0.0f;
-  }
-  Chunk<T> c;
-#pragma unroll
-  for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = u32x4{0, 0, 0, 0};
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const int64_t r = at * 8 + e;
-    if (j >= p.J || r >= p.R) continue;
-    if constexpr (sizeof(T) == 4) c.w[e >> 2][e & 3] = ((const uint32_t*)w)[r * p.b_r];
-    else c.w[0][e >> 1] |= (uint32_t)((const uint16_t*)w)[r * p.b_r] << (16 * (e & 1));
+    ((float*)(image + row / 8 * S::kRow + KS * 64))[row % 8] = bias && in ? to_f(bias[j]) : 0.0f;
   }
   // 16-bit results leave 8 at a time: the rows of a read are 4 + 4 + 4 + 4, 8 apart
   const int place = sizeof(T) == 2 ? (row & ~31) + 16 * ((row >> 2) & 1) + 4 * ((row >> 3) & 3) + (row & 3) : row;
   put_chunk<T>(image + place * S::kRow + at * 16, S::kPlane, c);
+}
+template <typename T, bool GATED, int KS>
+__global__ __launch_bounds__(256) void image_kernel(ProductArgs p, char* images, uint32_t chunks) {
+  using S = Strip<T, KS, GATED>;
+  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
+  if (id >= chunks) return;
+  const uint32_t tile = id / (KS * 4 * S::kRows);
+  image_chunk<T, GATED, KS>(p, tile, id / (KS * 4) % S::kRows, id % (KS * 4), images + (size_t)tile * S::kImage);
 }
 
 // EXTRA: there is a residual (forward).
@@ -112,7 +107,7 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
       }
   };
   const T* const x_end = (const T*)p.a + (p.I - 1) * p.a_i + K;
-  fetch(tile0, 0);
+  if (images) fetch(tile0, 0);
   s16x8 a[NI][KS][kPlanes];
 #pragma unroll
   for (int u = 0; u < NI; u++) {
@@ -133,6 +128,9 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
   }
   u32x4 ex[NI][kRuns] = {}, ex_next[NI][kRuns] = {};
   if (EXTRA) load_extra(ex, tile0);
+  if (!images)  // all outputs are one tile: everyone makes its image
+    for (int id = threadIdx.x; id < S::kRows * KS * 4; id += 64 * kWaves)
+      image_chunk<T, GATED, KS>(p, 0, id / (KS * 4), id % (KS * 4), lds);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   int buffer = 0;
 
@@ -143,7 +141,7 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
         // every wave's part of this image is in LDS, and everyone has left the image before it
         barrier();
         const uint32_t next = tile + 1 < tile1 ? tile + 1 : tile;
-        fetch(next, buffer ^ 1);
+        if (images) fetch(next, buffer ^ 1);
         if (EXTRA) load_extra(ex_next, next);
         const int64_t j0 = (int64_t)tile * kOut;
         const char* image = lds + buffer * S::kImage;
@@ -255,7 +253,7 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
 template <typename T, bool GATED, int KS>
 size_t image_bytes(int64_t J) {
   using S = Strip<T, KS, GATED>;
-  return (size_t)((J + S::kOut - 1) / S::kOut) * S::kImage;
+  return J > S::kOut ? (size_t)((J + S::kOut - 1) / S::kOut) * S::kImage : 0;
 }
 
 template <typename T, bool RCA, int EPI, bool GATED, int KS>
@@ -271,12 +269,16 @@ int launch_strip(const ProductArgs& p, char* scratch, hipStream_t stream) {
   parts = (tiles + part_tiles - 1) / part_tiles;
   const int64_t items = strips * parts;
   if (items > 0x7ffffff0 || chunks > 0x7fffffff) return 1;
-  hipLaunchKernelGGL((image_kernel<T, GATED, KS>), dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, stream, p,
-                     scratch, (uint32_t)chunks);
+  // one tile of weights is made by every workgroup itself: cheaper than a launch before this one
+  // (762048x3x64 in 32 bits: 67 us a call with it, 52 without)
+  const char* images = tiles > 1 ? scratch : nullptr;
+  if (images)
+    hipLaunchKernelGGL((image_kernel<T, GATED, KS>), dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, stream, p,
+                       scratch, (uint32_t)chunks);
   auto go = [&](auto extra) {
     hipLaunchKernelGGL((strip_kernel<T, RCA, EPI, GATED, decltype(extra)::value, KS>),
                        dim3((uint32_t)((items + 7) / 8 * 8)), dim3(64 * S::kWaves), 0, stream, p,
-                       (const char*)scratch, (uint32_t)strips, (uint32_t)parts, (uint32_t)part_tiles);
+                       images, (uint32_t)strips, (uint32_t)parts, (uint32_t)part_tiles);
   };
   if (EPI == EPI_DZ || (EPI == EPI_FORWARD && !GATED && p.extra)) go(Const<EPI != EPI_PLAIN && !(EPI == EPI_FORWARD && GATED)>());
   else go(Const<EPI == EPI_DZ>());

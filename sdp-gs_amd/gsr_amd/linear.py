@@ -30,11 +30,23 @@ def _check(rc, what):
         raise RuntimeError(f"{what} failed with status {rc}")
 
 
-def _checked(x, others, activation):
-    """Refuse what the kernels do not take (before any GPU work)."""
+def _fits(t, shape, x):
+    return t is None or (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is x.dtype
+                         and t.device == x.device)
+
+
+def _refuse(x, weight, weight_name, others, activation):
+    """Say what is wrong with a call that the kernels do not take (before any GPU work)."""
+    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
+        raise TypeError(f"x and {weight_name} must be tensors")
+    if x.dim() < 1 or weight.dim() != 2:
+        raise ValueError(f"x must be [..., K] and {weight_name} [N, K]")
+    N, K = weight.shape
+    if N < 1 or K < 1:
+        raise ValueError(f"{weight_name} [N, K] must not be empty")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
-    for name, t, shape in others:
+    for name, t, shape in [("x", x, x.shape[:-1] + (K,)), (weight_name, weight, (N, K))] + others(N, K):
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
@@ -49,36 +61,38 @@ def _checked(x, others, activation):
         raise ValueError(f"float32, float16 or bfloat16 expected, not {x.dtype}")
     if not x.is_cuda:
         raise RuntimeError("gsr fused products run on HIP tensors only (no CPU path)")
+    raise ValueError("gsr fused products: arguments not supported")
 
 
-def _weight_sizes(x, weight, name):
-    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
-        raise TypeError(f"x and {name} must be tensors")
-    if x.dim() < 1 or weight.dim() != 2:
-        raise ValueError(f"x must be [..., K] and {name} [N, K]")
-    N, K = (int(n) for n in weight.shape)
-    if N < 1 or K < 1:
-        raise ValueError(f"{name} [N, K] must not be empty")
-    return N, K
+def _base_fits(x, weight, activation):
+    return (isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and x.is_cuda
+            and x.dtype in DTYPES and activation in ACTIVATIONS and weight.dim() == 2
+            and x.dim() > 0 and x.shape[-1] == weight.shape[1] and weight.numel() > 0
+            and weight.dtype is x.dtype and weight.device == x.device)
 
 
 def _rows(t, n):
     """t [..., n] as a [M, n] matrix whose rows are contiguous (a copy only if it has to be)."""
     m = t.reshape(-1, n) if t.dim() != 2 else t
-    if (n > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < n):
+    row, col = m.stride()
+    if (col != 1 and n > 1) or (row < n and m.shape[0] > 1):
         m = m.contiguous()
     return m
 
 
 def _row_stride(m):
     """The distance between rows (a single row's stride means nothing)."""
-    return int(m.stride(0)) if m.shape[0] > 1 else int(m.shape[1])
+    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
 
 
 def _x_matrix(x, K):
     """x as (matrix, row stride, column stride): channel-major memory is taken as it lies."""
-    if x.dim() == 2 and K > 1 and x.shape[0] > 1 and x.stride(0) == 1 and x.stride(1) >= x.shape[0]:
-        return x, 1, int(x.stride(1))
+    if x.dim() == 2:
+        row, col = x.stride()
+        if col == 1 and row >= K:
+            return x, row, 1
+        if row == 1 and K > 1 and x.shape[0] > 1 and col >= x.shape[0]:
+            return x, 1, col
     m = _rows(x, K)
     return m, _row_stride(m), 1
 
@@ -88,7 +102,7 @@ def _ptr(t):
 
 
 def _scratch(nbytes, device):
-    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _wants_grad(*tensors):
@@ -104,7 +118,7 @@ class _Linear(torch.autograd.Function):
         w = _rows(weight, K)
         b = None if bias is None else bias.contiguous()
         r = None if residual is None else _rows(residual, N)
-        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        y = x.new_empty(x.shape[:-1] + (N,))
         if M:
             L = _lib.load()
             scratch = _scratch(L.gsr_linear_scratch_bytes(DTYPES[x.dtype], M, K, N), x.device)
@@ -112,7 +126,7 @@ class _Linear(torch.autograd.Function):
                 _check(L.gsr_linear(
                     DTYPES[x.dtype], M, K, N, xm.data_ptr(), x_row, x_col, w.data_ptr(),
                     _row_stride(w), _ptr(b), _ptr(r), 0 if r is None else _row_stride(r), act,
-                    y.data_ptr(), N, scratch.data_ptr(), _lib.raw_stream(x.device)), "gsr_linear")
+                    y.data_ptr(), N, _ptr(scratch), _lib.raw_stream(x.device)), "gsr_linear")
         if ctx is not None:
             ctx.save_for_backward(xm, w, b)
             ctx.args = (x.shape, x_row, x_col, act)
@@ -138,7 +152,7 @@ class _Linear(torch.autograd.Function):
                 _check(L.gsr_linear_backward(
                     DTYPES[kind], M, K, N, xm.data_ptr(), x_row, x_col, w.data_ptr(),
                     _row_stride(w), _ptr(b), act, g.data_ptr(), _row_stride(g), _ptr(dx), _ptr(dw),
-                    _ptr(db), scratch.data_ptr(), _lib.raw_stream(dev)), "gsr_linear_backward")
+                    _ptr(db), _ptr(scratch), _lib.raw_stream(dev)), "gsr_linear_backward")
         return dx, dw, db, dy if need_r else None, None
 
 
@@ -153,7 +167,7 @@ class _Gated(torch.autograd.Function):
             wg, wu = wg.contiguous(), wu.contiguous()
         bg = None if gate_bias is None else gate_bias.contiguous()
         bu = None if up_bias is None else up_bias.contiguous()
-        h = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        h = x.new_empty(x.shape[:-1] + (N,))
         if M:
             L = _lib.load()
             scratch = _scratch(L.gsr_gated_scratch_bytes(DTYPES[x.dtype], M, K, N), x.device)
@@ -161,7 +175,7 @@ class _Gated(torch.autograd.Function):
                 _check(L.gsr_gated(
                     DTYPES[x.dtype], M, K, N, xm.data_ptr(), _row_stride(xm), wg.data_ptr(),
                     wu.data_ptr(), _row_stride(wg), _ptr(bg), _ptr(bu), act, h.data_ptr(), N,
-                    scratch.data_ptr(), _lib.raw_stream(x.device)), "gsr_gated")
+                    _ptr(scratch), _lib.raw_stream(x.device)), "gsr_gated")
         if ctx is not None:
             ctx.save_for_backward(xm, wg, wu, bg, bu)
             ctx.args = (x.shape, act)
@@ -188,7 +202,7 @@ class _Gated(torch.autograd.Function):
                 _check(L.gsr_gated_backward(
                     DTYPES[kind], M, K, N, xm.data_ptr(), _row_stride(xm), wg.data_ptr(),
                     wu.data_ptr(), _row_stride(wg), _ptr(bg), _ptr(bu), act, g.data_ptr(),
-                    _row_stride(g), _ptr(dx), _ptr(dw), _ptr(db), scratch.data_ptr(),
+                    _row_stride(g), _ptr(dx), _ptr(dw), _ptr(db), _ptr(scratch),
                     _lib.raw_stream(dev)), "gsr_gated_backward")
         return (dx, dw[0] if need[1] else None, dw[1] if need[2] else None,
                 db[0] if need[3] else None, db[1] if need[4] else None, None)
@@ -197,9 +211,10 @@ class _Gated(torch.autograd.Function):
 def fused_linear(x, weight, bias=None, *, activation="none", residual=None):
     """activation(x @ weight.T + bias) + residual.  x [..., K], weight [N, K], bias [N], residual
     [..., N] (the result's shape); differentiable once in each of them."""
-    N, K = _weight_sizes(x, weight, "weight")
-    _checked(x, [("x", x, x.shape[:-1] + (K,)), ("weight", weight, (N, K)), ("bias", bias, (N,)),
-                 ("residual", residual, x.shape[:-1] + (N,))], activation)
+    if not (_base_fits(x, weight, activation) and _fits(bias, weight.shape[:1], x)
+            and _fits(residual, x.shape[:-1] + weight.shape[:1], x)):
+        _refuse(x, weight, "weight", lambda N, K: [
+            ("bias", bias, (N,)), ("residual", residual, x.shape[:-1] + (N,))], activation)
     if not _wants_grad(x, weight, bias, residual):
         return _Linear.forward(None, x, weight, bias, residual, ACTIVATIONS[activation])
     return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation])
@@ -208,10 +223,14 @@ def fused_linear(x, weight, bias=None, *, activation="none", residual=None):
 def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, activation="silu"):
     """activation(x @ gate_weight.T + gate_bias) * (x @ up_weight.T + up_bias), both products in
     one pass over x.  x [..., K], weights [N, K], biases [N]; differentiable once in each."""
-    N, K = _weight_sizes(x, gate_weight, "gate_weight")
-    _checked(x, [("x", x, x.shape[:-1] + (K,)), ("gate_weight", gate_weight, (N, K)),
-                 ("up_weight", up_weight, (N, K)), ("gate_bias", gate_bias, (N,)),
-                 ("up_bias", up_bias, (N,))], activation)
+    if not (_base_fits(x, gate_weight, activation) and up_weight is not None
+            and _fits(up_weight, gate_weight.shape, x) and _fits(gate_bias, gate_weight.shape[:1], x)
+            and _fits(up_bias, gate_weight.shape[:1], x)):
+        if up_weight is None:
+            raise TypeError("up_weight must be a tensor")
+        _refuse(x, gate_weight, "gate_weight", lambda N, K: [
+            ("up_weight", up_weight, (N, K)), ("gate_bias", gate_bias, (N,)),
+            ("up_bias", up_bias, (N,))], activation)
     if not _wants_grad(x, gate_weight, up_weight, gate_bias, up_bias):
         return _Gated.forward(None, x, gate_weight, up_weight, gate_bias, up_bias,
                               ACTIVATIONS[activation])

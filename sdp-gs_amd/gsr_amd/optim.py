@@ -34,6 +34,7 @@ MAX_TENSORS = 16  # GSR_ADAM_MAX_TENSORS
 
 _NORMS = {math.inf: 0, 1.0: 1, 2.0: 2}  # GSR_NORM_INF / 1 / 2
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # GSR_F32 / F16 / BF16
+_SIZES = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
 
 
 def _dense(t):
@@ -56,43 +57,43 @@ def _norm_code(norm_type):
     return _NORMS[float(norm_type)]
 
 
-def _nonempty(tensors):
-    """The tensors that hold elements, each checked."""
-    kept = []
-    device = tensors[0].device if tensors else None
-    for t in tensors:
-        if t.layout is not torch.strided:
-            raise RuntimeError("gradient norm: sparse gradients are not supported")
-        if t.dtype not in _DTYPES:
-            raise ValueError(f"gradient norm: float32, float16 or bfloat16 expected, not {t.dtype}")
-        if not t.is_cuda:
-            raise RuntimeError("gradient norm: HIP tensors only (no CPU path)")
-        if t.device != device:
-            raise ValueError("gradient norm: every gradient must be on one device")
-        if t.numel():
-            kept.append(t)
-    return kept
-
-
 class _CTensors:
-    """The tensors as the C entries take them; one with gaps between its elements as a copy."""
+    """The tensors that hold elements, checked, as the C entries take them; one with gaps between
+    its elements as a copy.  (Each attribute of each tensor is asked for once: a head has many.)"""
 
     def __init__(self, tensors):
-        self.tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
+        if any([t.is_sparse for t in tensors]):
+            raise RuntimeError("gradient norm: sparse gradients are not supported")
+        kinds = [t.dtype for t in tensors]
+        for kind in set(kinds):
+            if kind not in _DTYPES:
+                raise ValueError(f"gradient norm: float32, float16 or bfloat16 expected, not {kind}")
+        devices = {t.get_device() for t in tensors}
+        if len(devices) > 1:
+            raise ValueError("gradient norm: every gradient must be on one device")
+        if -1 in devices:
+            raise RuntimeError("gradient norm: HIP tensors only (no CPU path)")
+        numel = [t.numel() for t in tensors]
+        if 0 in numel:
+            keep = [i for i, m in enumerate(numel) if m]
+            tensors, kinds, numel = ([v[i] for i in keep] for v in (tensors, kinds, numel))
+        self.given = tensors
         self.n = n = len(tensors)
+        if not n:
+            return
+        self.tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
         self.pointers = [t.data_ptr() for t in self.tensors]
-        self.args = ((ctypes.c_void_p * n)(*self.pointers),
-                     (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
-                     (ctypes.c_int * n)(*[_DTYPES[t.dtype] for t in tensors]))
+        self.ends = [p + m * _SIZES[k] for p, m, k in zip(self.pointers, numel, kinds)]
+        self.args = ((ctypes.c_void_p * n)(*self.pointers), (ctypes.c_int64 * n)(*numel),
+                     (ctypes.c_int * n)(*[_DTYPES[k] for k in kinds]))
         self.device = tensors[0].device
-        self.scratch = torch.empty(int(_lib.load().gsr_grad_norm_scratch_bytes(n)),
-                                   dtype=torch.uint8, device=self.device)
+        self.scratch = torch.empty(_lib.load().gsr_grad_norm_scratch_bytes(n), dtype=torch.uint8,
+                                   device=self.device)
         self.norm = torch.empty((), dtype=torch.float32, device=self.device)
 
 
-def _norm_and_scale(tensors, norm_code, max_norm, scale=None):
+def _norm_and_scale(c, norm_code, max_norm, scale=None):
     """gsr_grad_norm on the current stream: the norm (and `scale`, a one-float tensor)."""
-    c = _CTensors(tensors)
     with _lib.on_device(c.device):
         rc = _lib.load().gsr_grad_norm(c.n, *c.args, norm_code, float(max_norm), c.norm.data_ptr(),
                                        None if scale is None else scale.data_ptr(),
@@ -108,24 +109,23 @@ def grad_norm(tensors, norm_type=2.0):
     device (not synchronised).  Any number of tensors, of mixed types, strides and sizes; sums in
     64 bits, the same tensors give the same bits.  No tensors (or only empty ones): 0."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    code, kept = _norm_code(norm_type), _nonempty(tensors)
-    if not kept:
+    code, c = _norm_code(norm_type), _CTensors(tensors)
+    if not c.n:
         return torch.zeros((), device=tensors[0].device if tensors else "cpu")
-    return _norm_and_scale(kept, code, math.inf)
+    return _norm_and_scale(c, code, math.inf)
 
 
-def _refuse_overlap(grads, c):
+def _refuse_overlap(c):
     """Two workgroups may not scale the same memory.  Gradients with gaps are scaled in copies, so
     only their overlap with one that is scaled in place counts."""
     spans = []
-    for t, own, start in zip(grads, c.tensors, c.pointers):
-        if t is own:
-            spans.append((start, start + t.numel() * t.element_size(), True))
-            continue
-        if 0 in [s for n, s in zip(t.shape, t.stride()) if n > 1]:
-            raise ValueError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        spans.append((t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size(), False))
+    for t, own, start, end in zip(c.given, c.tensors, c.pointers, c.ends):
+        if t is not own:
+            if 0 in [s for n, s in zip(t.shape, t.stride()) if n > 1]:
+                raise ValueError("clip_grad_norm_: an expanded gradient cannot be scaled in place")
+            last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+            start, end = t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+        spans.append((start, end, t is own))
     spans.sort()
     end_dense = end_any = 0
     for start, end, dense in spans:
@@ -149,22 +149,19 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         raise ValueError(f"max_norm must be at least 0, not {max_norm}")
     code = _norm_code(norm_type)
     grads = [g for g in [p.grad for p in parameters] if g is not None]
-    kept = _nonempty(grads)
-    if not kept:
+    c = _CTensors(grads)
+    if not c.n:
         return torch.zeros((), device=grads[0].device if grads else "cpu")
-    c = _CTensors(kept)
-    _refuse_overlap(kept, c)
-    if error_if_nonfinite:
-        norm = _norm_and_scale(kept, code, math.inf)
-        if not bool(torch.isfinite(norm)):
-            raise RuntimeError(f"The total norm of order {norm_type} is non-finite, so it cannot "
-                               "be clipped")
+    _refuse_overlap(c)
+    if error_if_nonfinite and not bool(torch.isfinite(_norm_and_scale(c, code, math.inf))):
+        raise RuntimeError(f"The total norm of order {norm_type} is non-finite, so it cannot "
+                           "be clipped")
     with _lib.on_device(c.device):
         rc = _lib.load().gsr_clip_grads(c.n, *c.args, code, max_norm, c.norm.data_ptr(),
                                         c.scratch.data_ptr(), _lib.raw_stream(c.device))
     if rc != 0:
         raise RuntimeError(f"gsr_clip_grads failed with status {rc}")
-    for t, own in zip(kept, c.tensors):
+    for t, own in zip(c.given, c.tensors):
         if t is not own:  # a gradient with gaps: its scaled copy goes back
             t.copy_(own)
     return c.norm
@@ -237,10 +234,10 @@ class FusedAdam(torch.optim.Adam):
         parameter (dim 0), end_rows(h) finishes.  The row ranges must cover every row exactly
         once; the result is bitwise the one of step() (the update is elementwise)."""
         self._resolve_pending()
-        kept = []
+        grads = None
         if self.max_grad_norm is not None:  # refused before any step count advances
-            kept = _nonempty([p.grad for group in self.param_groups for p in group["params"]
-                              if p.grad is not None])
+            grads = _CTensors([p.grad for group in self.param_groups for p in group["params"]
+                               if p.grad is not None])
         batches = {}
         for group in self.param_groups:
             beta1, beta2 = group["betas"]
@@ -295,9 +292,9 @@ class FusedAdam(torch.optim.Adam):
                 skips[dev] = (skip.data_ptr(), box)
         states = [self.state[it[0]] for its in batches.values() for it in its]
         scale = None
-        if kept:
-            scale = torch.empty(1, dtype=torch.float32, device=kept[0].device)
-            self.grad_norm = _norm_and_scale(kept, _NORMS[2.0], self.max_grad_norm, scale)
+        if grads is not None and grads.n:
+            scale = torch.empty(1, dtype=torch.float32, device=grads.device)
+            self.grad_norm = _norm_and_scale(grads, _NORMS[2.0], self.max_grad_norm, scale)
         return {"batches": batches, "skips": skips, "states": states, "issued": False,
                 "scale": scale}
 

@@ -222,7 +222,7 @@ def test_rows_beyond_the_last_are_untouched():
         for M, N in ((5, 20), (130, 131), (5001, 75)):
             d = ref.inputs(6, M, 24, N, t, "cuda")
             y = torch.full((M + 3, N + 8), 7.0, dtype=t, device="cuda")
-            scratch = torch.empty(L.gsr_linear_scratch_bytes(kind, M, 24, N), dtype=torch.uint8,
+            scratch = torch.empty(L.gsr_linear_scratch_bytes(kind, M, 24, N) + 1, dtype=torch.uint8,
                                   device="cuda")
             rc = L.gsr_linear(kind, M, 24, N, d["x"].data_ptr(), 24, 1, d["w0"].data_ptr(), 24,
                               d["b0"].data_ptr(), None, 0, 1, y.data_ptr(), N + 8,
@@ -355,7 +355,9 @@ def test_c_entries_refuse():
 
     assert lin(dtype=3) == lin(dtype=-1) == lin(act=4) == lin(act=-1) == 1
     assert lin(M=-1) == lin(K=0) == lin(N=0) == lin(K=1 << 40) == 1
-    assert lin(x=None) == lin(w=None) == lin(y=None) == lin(s=None) == 1
+    assert lin(x=None) == lin(w=None) == lin(y=None) == 1
+    assert lin(M=8192, N=80, yr=80, s=None) == 1  # this one needs scratch
+    assert L.gsr_linear_scratch_bytes(0, 8192, 6, 80) > 0 == L.gsr_linear_scratch_bytes(0, 4, 6, 8)
     assert lin(xr=5) == lin(xc=2) == lin(wr=5) == lin(yr=7) == lin(r=p, rr=7) == 1
     assert lin(xr=1, xc=3) == 1
     assert lin(M=0, x=None, y=None) == 0
@@ -365,7 +367,7 @@ def test_c_entries_refuse():
     assert L.gsr_gated(0, 4, 6, 8, p, 6, p, None, 6, None, None, 3, p, 8, p, None) == 1
     assert L.gsr_gated(0, 4, 6, 8, p, 5, p, p, 6, None, None, 3, p, 8, p, None) == 1
     assert L.gsr_gated_backward(0, 4, 6, 8, p, 6, p, p, 6, None, None, 3, None, 8, p, p, p, p, None) == 1
-    assert L.gsr_gated(0, 4, 6, 8, p, 6, p, p, 6, None, None, 3, p, 8, None, None) == 1
+    assert L.gsr_gated(0, 8192, 6, 80, p, 6, p, p, 6, None, None, 3, p, 80, None, None) == 1
     assert L.gsr_linear_scratch_bytes(0, -1, 6, 8) == L.gsr_gated_scratch_bytes(3, 4, 6, 8) == 0
     assert L.gsr_linear_backward_scratch_bytes(9, 4, 6, 8, 1, 1) == 0
     assert L.gsr_gated_backward_scratch_bytes(0, -4, 6, 8, 1) == 0
