@@ -641,29 +641,42 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
   });
 }
 
-template <typename T, bool RCA, bool RCB, int EPI, bool GATED, int BI, int WI, int BJ, int WJ>
-int launch_product(const ProductArgs& p, int64_t splits, hipStream_t stream) {
+// Whether every 16-byte chunk of the operands is aligned, so that steps can go straight to LDS.
+template <typename T, bool RCA, bool RCB>
+bool takes_direct(const ProductArgs& p) {
+  const uint64_t bits = (uint64_t)p.a | (uint64_t)p.b[0] | (uint64_t)p.b[1] |
+                        (uint64_t)((RCA ? p.a_i : p.a_r) | (RCB ? p.b_j : p.b_r) | p.a_segment) * sizeof(T);
+  return sizeof(T) == 2 && bits % 16 == 0;
+}
+
+template <typename T, bool RCA, bool RCB, int EPI, bool GATED, bool DIRECT, int BI, int WI, int BJ, int WJ>
+int launch_tiles(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   constexpr int kOut = GATED ? BJ / 2 : BJ;
   const int64_t ti = (p.I + BI - 1) / BI, tj = (p.J + kOut - 1) / kOut;
   if (ti > 0x7fffffff / tj || ti * tj > 0x7ffffff0 / splits) return 1;
   const int64_t total = ti * tj * splits, grid = (total + 7) / 8 * 8;
-  // straight to LDS where every 16-byte chunk is aligned
-  const uint64_t bits = (uint64_t)p.a | (uint64_t)p.b[0] | (uint64_t)p.b[1] |
-                        (uint64_t)((RCA ? p.a_i : p.a_r) | (RCB ? p.b_j : p.b_r) | p.a_segment) * sizeof(T);
-  auto go = [&](auto direct) {
-    hipLaunchKernelGGL((product_kernel<T, RCA, RCB, EPI, GATED, decltype(direct)::value, BI, WI, BJ, WJ>),
-                       dim3((uint32_t)grid), dim3(64 * WI * WJ), 0, stream, p, (uint32_t)ti, (uint32_t)tj,
-                       (uint32_t)splits);
-  };
-  if (sizeof(T) == 2 && bits % 16 == 0) go(Const<sizeof(T) == 2>());
-  else go(Const<0>());
+  hipLaunchKernelGGL((product_kernel<T, RCA, RCB, EPI, GATED, DIRECT, BI, WI, BJ, WJ>), dim3((uint32_t)grid),
+                     dim3(64 * WI * WJ), 0, stream, p, (uint32_t)ti, (uint32_t)tj, (uint32_t)splits);
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
+template <typename T, bool RCA, bool RCB, int EPI, bool GATED, int BI, int WI, int BJ, int WJ>
+int launch_product(const ProductArgs& p, int64_t splits, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if (takes_direct<T, RCA, RCB>(p))
+      return launch_tiles<T, RCA, RCB, EPI, GATED, true, BI, WI, BJ, WJ>(p, splits, stream);
+  return launch_tiles<T, RCA, RCB, EPI, GATED, false, BI, WI, BJ, WJ>(p, splits, stream);
+}
 
-// The tile by the size of C: 128 x 128 where there are outputs for it, 128 x 64 for narrow
-// results, 64 x 64 where the larger ones would leave CUs without work.
+// The tile by the size of C: 256 x 256 where one a CU keeps it busy (operands straight to LDS),
+// 128 x 128 where there are outputs for it, 128 x 64 for narrow results, 64 x 64 where the larger
+// ones would leave CUs without work.
 template <typename T, bool RCA, bool RCB, int EPI>
 int launch_linear(const ProductArgs& p, int64_t splits, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    const int64_t huge = (p.I + 255) / 256 * ((p.J + 255) / 256) * splits;
+    if (p.J > 128 && huge >= 256 && takes_direct<T, RCA, RCB>(p))
+      return launch_tiles<T, RCA, RCB, EPI, false, true, 256, 4, 256, 2>(p, splits, stream);
+  }
   const int64_t large = (p.I + 127) / 128 * ((p.J + 127) / 128) * splits;
   if (p.J > 64 && large >= 256) return launch_product<T, RCA, RCB, EPI, false, 128, 2, 128, 2>(p, splits, stream);
   if (p.J <= 64 && (p.I + 127) / 128 * splits >= 256)

@@ -16,11 +16,11 @@ namespace gsr {
 // waves of 16 kNI rows of x, for up to 32 KS inputs; kGroups workgroups to a CU, as many as its
 // registers and LDS hold.
 template <typename T, int KS, bool GATED> struct Strip {
-  static constexpr bool kSplit = sizeof(T) == 4;
+  static constexpr bool kSplit = sizeof(T) == 4, kWide = kSplit && KS > 6;
   static constexpr int kNI = kSplit && KS > 4 ? 1 : 2;  // three parts of x fill the registers
-  static constexpr int kWaves = kSplit && KS > 6 ? 8 : 4;
-  static constexpr int kRows = kSplit ? 32 : 64;
-  static constexpr int kGroups = kSplit && KS > 6 ? 1 : kSplit || KS > 2 ? 2 : 3;
+  static constexpr int kWaves = kWide && GATED ? 8 : 4;
+  static constexpr int kRows = !kSplit || KS == 1 ? 64 : kWide && !GATED ? 16 : 32;
+  static constexpr int kGroups = kWide && GATED ? 1 : kSplit || KS > 2 ? 2 : 3;
   static constexpr int kOut = GATED ? kRows / 2 : kRows;  // outputs of a tile
   // Bytes of a row: the 32 of padding turn it by two of the 16 bank groups, so that the lanes that
   // a 16-byte read takes together (0-3, 12-15, 20-23, 24-27 and so on) hit different ones.  The
@@ -37,7 +37,11 @@ __device__ __forceinline__ void image_chunk(const ProductArgs& p, uint32_t tile,
   const bool second = GATED && row >= S::kOut;
   const int64_t j = (int64_t)tile * S::kOut + (second ? row - S::kOut : row);
   const bool in = j < p.J;
-  Chunk<T> c = load_tail((const T*)p.b[second ? 1 : 0] + (in ? j : 0) * p.b_j, at * 8, p.b_r, p.R);
+  const T* w = (const T*)p.b[second ? 1 : 0];
+  const T* row_of_w = w + (in ? j : 0) * p.b_j;
+  const int64_t whole = (p.J - 1) * p.b_j + p.R;  // elements, if rows are contiguous
+  Chunk<T> c = p.b_r == 1 && whole >= 8 ? load_row_end(row_of_w, at * 8, p.R, w + whole)
+                                        : load_tail(row_of_w, at * 8, p.b_r, p.R);
 #pragma unroll
   for (int k = 0; k < Operand<T>::kRaw; k++) c.w[k] = in ? c.w[k] : u32x4{0, 0, 0, 0};
   if (at == 0) {
@@ -251,9 +255,13 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
 }
 
 template <typename T, bool GATED, int KS>
+bool needs_images(int64_t J) {
+  return KS > 2 || J > Strip<T, KS, GATED>::kOut;
+}
+template <typename T, bool GATED, int KS>
 size_t image_bytes(int64_t J) {
   using S = Strip<T, KS, GATED>;
-  return J > S::kOut ? (size_t)((J + S::kOut - 1) / S::kOut) * S::kImage : 0;
+  return needs_images<T, GATED, KS>(J) ? (size_t)((J + S::kOut - 1) / S::kOut) * S::kImage : 0;
 }
 
 template <typename T, bool RCA, int EPI, bool GATED, int KS>
@@ -269,9 +277,10 @@ int launch_strip(const ProductArgs& p, char* scratch, hipStream_t stream) {
   parts = (tiles + part_tiles - 1) / part_tiles;
   const int64_t items = strips * parts;
   if (items > 0x7ffffff0 || chunks > 0x7fffffff) return 1;
-  // one tile of weights is made by every workgroup itself: cheaper than a launch before this one
-  // (762048x3x64 in 32 bits: 67 us a call with it, 52 without)
-  const char* images = tiles > 1 ? scratch : nullptr;
+  // one small tile of weights is made by every workgroup itself: cheaper than a launch before this
+  // one (762048x3x64 in 32 bits: 67 us a call with it, 57 without); not a large one (bf16
+  // 762048x256x64: 101 us with it, 142 without)
+  const char* images = needs_images<T, GATED, KS>(p.J) ? scratch : nullptr;
   if (images)
     hipLaunchKernelGGL((image_kernel<T, GATED, KS>), dim3((uint32_t)((chunks + 255) / 256)), dim3(256), 0, stream, p,
                        scratch, (uint32_t)chunks);
@@ -285,8 +294,11 @@ int launch_strip(const ProductArgs& p, char* scratch, hipStream_t stream) {
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-// Strips for up to 256 inputs and enough rows that every CU has one.
-inline bool takes_strips(int64_t I, int64_t R) { return R <= 256 && I >= 4096; }
+// Strips for up to 256 inputs and enough rows that every CU has one of 128: below that the tiled
+// kernel, which needs no images, is as fast or faster (us, strips : tiles; bf16 20011x256x512 gated
+// 26 : 23, 5000x256x512 11 : 7, fp32 20011x193x333 33 : 30; but bf16 190512x256x512 gated 121 : 213,
+// 762048x256x512 345 : 480, fp32 262144x256x256 220 : 246).
+inline bool takes_strips(int64_t I, int64_t R) { return R <= 256 && I >= 32768; }
 
 // f(integral constant KS) for R inputs.
 template <typename F>

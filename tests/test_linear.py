@@ -46,8 +46,10 @@ def _run(d, act, grads=True):
 # wide weights, many rows against a narrow output
 SIZES = [(1, 1, 1), (1, 512, 512), (2, 3, 5), (5, 4096, 33), (17, 129, 1000), (31, 64, 64), (33, 100, 66),
          (64, 64, 64), (65, 65, 65), (127, 31, 129), (128, 128, 128), (129, 256, 257),
-         (300, 7, 1), (512, 1, 16), (777, 161, 203), (2049, 96, 40), (3000, 33, 130), (4100, 31, 70), (4097, 63, 33),
-         (5000, 100, 129), (4130, 201, 65)]
+         (300, 7, 1), (512, 1, 16), (777, 161, 203), (2049, 96, 40), (3000, 33, 130), (4100, 31, 70), (5000, 100, 129),
+         # enough rows for the kernel that keeps its rows: 1, 2, 4, 6 and 8 steps of 32 inputs
+         (32769, 31, 70), (32800, 3, 64), (33000, 63, 33), (32768, 128, 64), (32771, 161, 203),
+         (32900, 256, 130), (33001, 250, 40)]
 
 
 @gpu
@@ -82,7 +84,7 @@ def test_activations_far_from_zero(act, t):
 @gpu
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("K", [1, 3, 16, 61])
-@pytest.mark.parametrize("M", [1, 2, 63, 1000, 4101])
+@pytest.mark.parametrize("M", [1, 2, 63, 1000, 33003])
 def test_channel_major_input(M, K, t):
     """A [K,H,W] image read as its transpose, in place; its gradient reaches the image."""
     d = ref.inputs(M + K, M, K, 40, t, "cuda")
@@ -183,7 +185,7 @@ def test_no_rows(t):
 
 
 @gpu
-@pytest.mark.parametrize("M", [3, 300, 5000])
+@pytest.mark.parametrize("M", [3, 300, 33000])
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 def test_infinities_and_nan_stay_where_they_are(t, M):
     """A row with an infinity or a NaN spoils that row as 64-bit arithmetic says, and no other."""
@@ -219,7 +221,7 @@ def test_rows_beyond_the_last_are_untouched():
     from gsr_amd import _lib
     L = _lib.load()
     for kind, t in ((0, torch.float32), (2, torch.bfloat16)):
-        for M, N in ((5, 20), (130, 131), (5001, 75)):
+        for M, N in ((5, 20), (130, 131), (33001, 75)):
             d = ref.inputs(6, M, 24, N, t, "cuda")
             y = torch.full((M + 3, N + 8), 7.0, dtype=t, device="cuda")
             scratch = torch.empty(L.gsr_linear_scratch_bytes(kind, M, 24, N) + 1, dtype=torch.uint8,
@@ -356,8 +358,8 @@ def test_c_entries_refuse():
     assert lin(dtype=3) == lin(dtype=-1) == lin(act=4) == lin(act=-1) == 1
     assert lin(M=-1) == lin(K=0) == lin(N=0) == lin(K=1 << 40) == 1
     assert lin(x=None) == lin(w=None) == lin(y=None) == 1
-    assert lin(M=8192, N=80, yr=80, s=None) == 1  # this one needs scratch
-    assert L.gsr_linear_scratch_bytes(0, 8192, 6, 80) > 0 == L.gsr_linear_scratch_bytes(0, 4, 6, 8)
+    assert lin(M=40000, N=80, yr=80, s=None) == 1  # this one needs scratch
+    assert L.gsr_linear_scratch_bytes(0, 40000, 6, 80) > 0 == L.gsr_linear_scratch_bytes(0, 4, 6, 8)
     assert lin(xr=5) == lin(xc=2) == lin(wr=5) == lin(yr=7) == lin(r=p, rr=7) == 1
     assert lin(xr=1, xc=3) == 1
     assert lin(M=0, x=None, y=None) == 0
@@ -367,7 +369,7 @@ def test_c_entries_refuse():
     assert L.gsr_gated(0, 4, 6, 8, p, 6, p, None, 6, None, None, 3, p, 8, p, None) == 1
     assert L.gsr_gated(0, 4, 6, 8, p, 5, p, p, 6, None, None, 3, p, 8, p, None) == 1
     assert L.gsr_gated_backward(0, 4, 6, 8, p, 6, p, p, 6, None, None, 3, None, 8, p, p, p, p, None) == 1
-    assert L.gsr_gated(0, 8192, 6, 80, p, 6, p, p, 6, None, None, 3, p, 80, None, None) == 1
+    assert L.gsr_gated(0, 40000, 6, 80, p, 6, p, p, 6, None, None, 3, p, 80, None, None) == 1
     assert L.gsr_linear_scratch_bytes(0, -1, 6, 8) == L.gsr_gated_scratch_bytes(3, 4, 6, 8) == 0
     assert L.gsr_linear_backward_scratch_bytes(9, 4, 6, 8, 1, 1) == 0
     assert L.gsr_gated_backward_scratch_bytes(0, -4, 6, 8, 1) == 0
