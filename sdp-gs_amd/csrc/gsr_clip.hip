@@ -19,7 +19,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 8192;  // elements: 8 vectors of 4 per lane
+constexpr int kChunk = 8192;  // elements: two batches of a lane in 32 bits, one in 16
 constexpr int kGrid = 2048;   // workgroups (and partial sums) of a launch: 8 per CU
 constexpr int kTensors = GSR_CLIP_LAUNCH_TENSORS;
 
@@ -31,15 +31,20 @@ struct Tensors {
   uint8_t dtype[kTensors];
 };
 
-template <typename T> __device__ __forceinline__ float load_f(const T* p);
-template <> __device__ __forceinline__ float load_f<float>(const float* p) { return *p; }
-template <> __device__ __forceinline__ float load_f<__half>(const __half* p) { return __half2float(*p); }
-template <> __device__ __forceinline__ float load_f<__hip_bfloat16>(const __hip_bfloat16* p) {
-  return __bfloat162float(*p);
-}
-__device__ __forceinline__ void store_f(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half(v); }
-__device__ __forceinline__ void store_f(__hip_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f<__hip_bfloat16>(__hip_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half(v); }
+template <> __device__ __forceinline__ __hip_bfloat16 from_f<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
+
+// 16 bytes of elements at any element's address (a gradient may start anywhere).
+template <typename T> struct __attribute__((packed, aligned(2))) Vec {
+  T e[16 / sizeof(T)];
+};
+constexpr int kBatch = 4;  // vectors of a lane in flight
 
 template <int NORM>
 __device__ __forceinline__ double join(double a, double b) {
@@ -64,9 +69,28 @@ __device__ double block_join(double v) {
 }
 
 template <typename T, int NORM>
-__device__ __forceinline__ double chunk_sum(const T* g, int64_t n) {
+__device__ __forceinline__ double chunk_sum(const T* g, int n) {
+  constexpr int V = 16 / sizeof(T), kStep = kBatch * kThreads * V;
   double v = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) v = join<NORM>(v, term<NORM>(load_f(g + i)));
+  int i = 0;
+  for (; i + kStep <= n; i += kStep) {
+    Vec<T> w[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; u++) w[u] = *(const Vec<T>*)(g + i + (u * kThreads + threadIdx.x) * V);
+#pragma unroll
+    for (int u = 0; u < kBatch; u++)
+#pragma unroll
+      for (int e = 0; e < V; e++) v = join<NORM>(v, term<NORM>(to_f(w[u].e[e])));
+  }
+  for (i += threadIdx.x * V; i < n; i += kThreads * V) {
+    if (i + V <= n) {
+      const Vec<T> w = *(const Vec<T>*)(g + i);
+#pragma unroll
+      for (int e = 0; e < V; e++) v = join<NORM>(v, term<NORM>(to_f(w.e[e])));
+    } else {
+      for (int e = i; e < n; e++) v = join<NORM>(v, term<NORM>(to_f(g[e])));
+    }
+  }
   return v;
 }
 
@@ -77,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(Tensors a, double* part)
   for (uint32_t c = blockIdx.x; c < a.chunk0[a.n]; c += gridDim.x) {
     while (c >= a.chunk0[t + 1]) t++;
     const int64_t at = (int64_t)(c - a.chunk0[t]) * kChunk;
-    const int64_t n = a.numel[t] - at < kChunk ? a.numel[t] - at : kChunk;
+    const int n = a.numel[t] - at < kChunk ? (int)(a.numel[t] - at) : kChunk;
     if (a.dtype[t] == GSR_F32) v = join<NORM>(v, chunk_sum<float, NORM>((const float*)a.g[t] + at, n));
     else if (a.dtype[t] == GSR_F16) v = join<NORM>(v, chunk_sum<__half, NORM>((const __half*)a.g[t] + at, n));
     else v = join<NORM>(v, chunk_sum<__hip_bfloat16, NORM>((const __hip_bfloat16*)a.g[t] + at, n));
@@ -110,8 +134,22 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const double* part, in
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_scale(T* g, int64_t n, float c) {
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) store_f(g + i, load_f(g + i) * c);
+__device__ __forceinline__ void chunk_scale(T* g, int n, float c) {
+  constexpr int V = 16 / sizeof(T), kStep = kBatch * kThreads * V;
+  int i = 0;
+  for (; i + kStep <= n; i += kStep) {
+    Vec<T> w[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; u++) w[u] = *(const Vec<T>*)(g + i + (u * kThreads + threadIdx.x) * V);
+#pragma unroll
+    for (int u = 0; u < kBatch; u++) {
+#pragma unroll
+      for (int e = 0; e < V; e++) w[u].e[e] = from_f<T>(to_f(w[u].e[e]) * c);
+      *(Vec<T>*)(g + i + (u * kThreads + threadIdx.x) * V) = w[u];
+    }
+  }
+  for (i += threadIdx.x * V; i < n; i += kThreads * V)
+    for (int e = i; e < n && e < i + V; e++) g[e] = from_f<T>(to_f(g[e]) * c);
 }
 
 template <int NORM>
@@ -125,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Tensors a, const double
   for (uint32_t c = blockIdx.x; c < a.chunk0[a.n]; c += gridDim.x) {
     while (c >= a.chunk0[t + 1]) t++;
     const int64_t at = (int64_t)(c - a.chunk0[t]) * kChunk;
-    const int64_t n = a.numel[t] - at < kChunk ? a.numel[t] - at : kChunk;
+    const int n = a.numel[t] - at < kChunk ? (int)(a.numel[t] - at) : kChunk;
     if (a.dtype[t] == GSR_F32) chunk_scale((float*)a.g[t] + at, n, s);
     else if (a.dtype[t] == GSR_F16) chunk_scale((__half*)a.g[t] + at, n, s);
     else chunk_scale((__hip_bfloat16*)a.g[t] + at, n, s);

@@ -48,14 +48,15 @@ __global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// Ranges of the summed rows for dw: enough 128 x 128 tiles to fill 256 CUs twice, each with at
-// least 256 rows and a whole number of the kernel's steps.
+// Ranges of the summed rows for dw: enough tiles to fill the 256 CUs, twice with 128 x 128 tiles,
+// once with 256 x 256, each with at least 256 rows and a whole number of the kernel's steps.
 struct Ranges {
   int64_t rows, count;
 };
-Ranges ranges_of(int64_t I, int64_t J, int64_t R) {
-  const int64_t t = (I + 127) / 128 * ((J + 127) / 128), want = (512 + t - 1) / t;
-  int64_t rows = up((R + want - 1) / want, 64);
+Ranges ranges_of(int64_t I, int64_t J, int64_t R, bool huge) {
+  const int64_t side = huge ? 256 : 128, want = huge ? 256 : 512;
+  const int64_t t = (I + side - 1) / side * ((J + side - 1) / side), n = (want + t - 1) / t;
+  int64_t rows = up((R + n - 1) / n, 64);  // one workgroup more than there is room for doubles the time
   if (rows < 256) rows = 256;
   return {rows, (R + rows - 1) / rows};
 }
@@ -79,12 +80,12 @@ int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64
     if (db) hipLaunchKernelGGL(zero_kernel<T>, dim3((I + 255) / 256), dim3(256), 0, stream, (T*)db, I);
     return hipGetLastError() == hipSuccess ? 0 : 2;
   }
-  const Ranges ranges = ranges_of(I, K, M);
-  const int64_t splits = ranges.count;
   ProductArgs p{};
   p.a = dz; p.a_i = 1; p.a_r = dz_row;
   p.b[0] = x; p.b_j = x_col; p.b_r = x_row;
   p.I = I; p.J = K; p.R = M; p.segments = 1;
+  const Ranges ranges = ranges_of(I, K, M, product_dw_huge<T>(p));
+  const int64_t splits = ranges.count;
   p.r_chunk = ranges.rows;
   p.part = (float*)scratch;
   p.part_sum = db ? p.part + splits * I * K : nullptr;
@@ -96,7 +97,10 @@ int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64
 }
 
 size_t partial_bytes(int64_t M, int64_t K, int64_t I) {
-  return M == 0 ? 0 : (size_t)ranges_of(I, K, M).count * I * (K + 1) * 4;
+  if (M == 0) return 0;
+  int64_t n = ranges_of(I, K, M, false).count;
+  if (takes_huge_dw(I, K) && ranges_of(I, K, M, true).count > n) n = ranges_of(I, K, M, true).count;
+  return (size_t)n * I * (K + 1) * 4;
 }
 
 // Scratch of a backward, in order: the pre-activation gradients, then what one product at a time

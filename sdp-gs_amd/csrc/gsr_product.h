@@ -264,26 +264,42 @@ struct Tile {
     else each(Const<2>());
   }
 
-  // All there and every row and base a multiple of 16 bytes: straight into LDS, 1 KB per
-  // instruction, each lane fetching the chunk that belongs where it writes (16-bit types).
+  // Every row and base a multiple of 16 bytes and no chunk across an end (16-bit types): straight
+  // into LDS, 1 KB per instruction, each lane fetching the chunk that belongs where it writes.  A
+  // chunk past an end is another one instead; where it is past r_end, clear() follows.
   static __device__ __forceinline__ void direct(char* lds, const T* base, const T* base1, int split, int64_t ld,
-                                                int64_t o0, int64_t O, int64_t r0) {
+                                                int64_t o0, int64_t O, int64_t r0, int64_t r_end) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto each = [&](auto whole) {
+#pragma unroll
+      for (int s = 0; s < kChunks; s++) {
+        const int q = s * THREADS + threadIdx.x, row = q / kPerRow, col = (q % kPerRow ^ swizzle(row)) * 8;
+        const T* p;
+        if (RC) {
+          const bool second = split && row >= split;
+          int64_t o = o0 + (second ? row - split : row);
+          o = o < O ? o : O - 1;
+          p = (second ? base1 : base) + o * ld + (decltype(whole)::value || r0 + col < r_end ? r0 + col : 0);
+        } else {
+          // the lane's own part of the address does not change from step to step
+          const int64_t c = o0 + col < O ? o0 + col : 0;
+          if (decltype(whole)::value) p = base + r0 * ld + (row * ld + c);
+          else p = base + (r0 + row < r_end ? r0 + row : r_end - 1) * ld + c;
+        }
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                         (__attribute__((address_space(3))) void*)(lds + (s * THREADS + wave * 64) * 16),
+                                         16, 0, 0);
+      }
+    };
+    if (r0 + kDepth <= r_end) each(Const<1>());
+    else each(Const<0>());
+  }
+  // Zeros for the chunks of a last step that are past r_end; each thread those that it fetched.
+  static __device__ __forceinline__ void clear(char* lds, int64_t r0, int64_t r_end) {
 #pragma unroll
     for (int s = 0; s < kChunks; s++) {
       const int q = s * THREADS + threadIdx.x, row = q / kPerRow, col = (q % kPerRow ^ swizzle(row)) * 8;
-      const T* p;
-      if (RC) {
-        const bool second = split && row >= split;
-        int64_t o = o0 + (second ? row - split : row);
-        o = o < O ? o : O - 1;
-        p = (second ? base1 : base) + o * ld + r0 + col;
-      } else {
-        p = base + (r0 + row) * ld + o0 + col;
-      }
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
-                                       (__attribute__((address_space(3))) void*)(lds + (s * THREADS + wave * 64) * 16),
-                                       16, 0, 0);
+      if (r0 + (RC ? col : row) >= r_end) *(u32x4*)(lds + q * 16) = u32x4{0, 0, 0, 0};
     }
   }
 
@@ -525,26 +541,29 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
 
   if constexpr (DIRECT) {
     // a step goes straight to LDS while the step before it is worked on
-    const bool columns = (RCA || i0 + BI <= p.I) && (RCB || j0 + kOut <= p.J);
     auto stage = [&](uint32_t it, int buffer) {
       at_step(it, [&](const T* a, const T* b, int64_t r0) {
-        if (columns && r0 + kDepth <= r_end) {
-          char* s = lds + buffer * (TA::kBytes + TB::kBytes);
-          TA::direct(s, a, nullptr, 0, lda, i0, p.I, r0);
-          TB::direct(s + TA::kBytes, b, (const T*)p.b[1], kSplit, ldb, j0, p.J, r0);
-        } else {
-          load(it);
-          store(buffer);
-        }
+        char* s = lds + buffer * (TA::kBytes + TB::kBytes);
+        TA::direct(s, a, nullptr, 0, lda, i0, p.I, r0, r_end);
+        TB::direct(s + TA::kBytes, b, (const T*)p.b[1], kSplit, ldb, j0, p.J, r0, r_end);
+      });
+    };
+    auto arrived = [&](uint32_t it, int buffer) {  // this wave's part of the step is in LDS
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      at_step(it, [&](const T*, const T*, int64_t r0) {
+        if (r0 + kDepth <= r_end) return;
+        char* s = lds + buffer * (TA::kBytes + TB::kBytes);
+        TA::clear(s, r0, r_end);
+        TB::clear(s + TA::kBytes, r0, r_end);
       });
     };
     stage(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    arrived(0, 0);
     for (uint32_t it = 0; it < total; it++) {
       barrier();  // every wave's part of this step is there, and everyone has left the other buffer
       if (it + 1 < total) stage(it + 1, (it + 1) & 1);
       compute(it & 1);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (it + 1 < total) arrived(it + 1, (it + 1) & 1);
     }
   } else if constexpr (kBuffers == 2) {
     load(0);
@@ -641,9 +660,12 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
   });
 }
 
-// Whether every 16-byte chunk of the operands is aligned, so that steps can go straight to LDS.
+// Whether every 16-byte chunk of the operands is aligned and within an end or past it, so that steps
+// can go straight to LDS.
 template <typename T, bool RCA, bool RCB>
 bool takes_direct(const ProductArgs& p) {
+  if ((RCA || RCB) && p.R % 8) return false;
+  if ((!RCA && p.I % 8) || (!RCB && p.J % 8)) return false;
   const uint64_t bits = (uint64_t)p.a | (uint64_t)p.b[0] | (uint64_t)p.b[1] |
                         (uint64_t)((RCA ? p.a_i : p.a_r) | (RCB ? p.b_j : p.b_r) | p.a_segment) * sizeof(T);
   return sizeof(T) == 2 && bits % 16 == 0;
@@ -667,6 +689,9 @@ int launch_product(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   return launch_tiles<T, RCA, RCB, EPI, GATED, false, BI, WI, BJ, WJ>(p, splits, stream);
 }
 
+// Whether a 16-bit weight gradient of I x J takes 256 x 256 tiles (if its operands are aligned).
+inline bool takes_huge_dw(int64_t I, int64_t J) { return I > 128 && J > 128; }  // 256 x 256 tiles
+
 // The tile by the size of C: 256 x 256 where one a CU keeps it busy (operands straight to LDS),
 // 128 x 128 where there are outputs for it, 128 x 64 for narrow results, 64 x 64 where the larger
 // ones would leave CUs without work.
@@ -674,7 +699,7 @@ template <typename T, bool RCA, bool RCB, int EPI>
 int launch_linear(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
     const int64_t huge = (p.I + 255) / 256 * ((p.J + 255) / 256) * splits;
-    if (p.J > 128 && huge >= 256 && takes_direct<T, RCA, RCB>(p))
+    if ((EPI == EPI_PARTIAL ? takes_huge_dw(p.I, p.J) : p.J > 128 && huge >= 256) && takes_direct<T, RCA, RCB>(p))
       return launch_tiles<T, RCA, RCB, EPI, false, true, 256, 4, 256, 2>(p, splits, stream);
   }
   const int64_t large = (p.I + 127) / 128 * ((p.J + 127) / 128) * splits;
@@ -697,5 +722,6 @@ template <typename T> int product_forward(const ProductArgs& p, bool gated, char
 template <typename T> int product_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s);
 template <typename T> int product_dx(const ProductArgs& p, char* scratch, hipStream_t s);
 template <typename T> int product_dw(const ProductArgs& p, int64_t splits, hipStream_t s);
+template <typename T> bool product_dw_huge(const ProductArgs& p);
 
 }  // namespace gsr

@@ -345,6 +345,10 @@ int forward_or_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s
       return launch_strips<T, true, EPI_PLAIN, false>(p, scratch, s);                                \
     return launch_linear<T, true, false, EPI_PLAIN>(p, 1, s);                                        \
   }                                                                                                  \
+  template <> bool product_dw_huge<T>(const ProductArgs& p) {                                        \
+    return sizeof(T) == 2 && takes_huge_dw(p.I, p.J) &&                                              \
+           (p.b_j == 1 ? takes_direct<T, false, false>(p) : takes_direct<T, false, true>(p));        \
+  }                                                                                                  \
   template <> int product_dw<T>(const ProductArgs& p, int64_t splits, hipStream_t s) {               \
     return p.b_j == 1 ? launch_linear<T, false, false, EPI_PARTIAL>(p, splits, s)                    \
                       : launch_linear<T, false, true, EPI_PARTIAL>(p, splits, s);                    \

@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -51,6 +52,12 @@ def _dense(t):
     return True
 
 
+def _without_gaps(t):
+    if t.layout is not torch.strided:
+        raise RuntimeError("gradient norm: sparse gradients are not supported")
+    return t if _dense(t) else t.contiguous()
+
+
 def _norm_code(norm_type):
     if isinstance(norm_type, str) or float(norm_type) not in _NORMS:
         raise ValueError(f"norm_type must be 1, 2 or inf, not {norm_type!r}")
@@ -62,8 +69,6 @@ class _CTensors:
     its elements as a copy.  (Each attribute of each tensor is asked for once: a head has many.)"""
 
     def __init__(self, tensors):
-        if any([t.is_sparse for t in tensors]):
-            raise RuntimeError("gradient norm: sparse gradients are not supported")
         kinds = [t.dtype for t in tensors]
         for kind in set(kinds):
             if kind not in _DTYPES:
@@ -81,7 +86,7 @@ class _CTensors:
         self.n = n = len(tensors)
         if not n:
             return
-        self.tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
+        self.tensors = [t if t.is_contiguous() else _without_gaps(t) for t in tensors]
         self.pointers = [t.data_ptr() for t in self.tensors]
         self.ends = [p + m * _SIZES[k] for p, m, k in zip(self.pointers, numel, kinds)]
         self.args = ((ctypes.c_void_p * n)(*self.pointers), (ctypes.c_int64 * n)(*numel),
@@ -118,6 +123,11 @@ def grad_norm(tensors, norm_type=2.0):
 def _refuse_overlap(c):
     """Two workgroups may not scale the same memory.  Gradients with gaps are scaled in copies, so
     only their overlap with one that is scaled in place counts."""
+    if all(map(operator.is_, c.given, c.tensors)):
+        spans = sorted(zip(c.pointers, c.ends))
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("clip_grad_norm_: two gradients share memory (the same one twice?)")
+        return
     spans = []
     for t, own, start, end in zip(c.given, c.tensors, c.pointers, c.ends):
         if t is not own:
