@@ -38,7 +38,8 @@ int gsr_linear(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_
 
 /* Gradients of gsr_linear: with z = x w^T + bias (computed again, so a forward keeps nothing)
  * and dz = dy act'(z): dx = dz w [M,K], dw = dz^T x [N,K], dbias = the column sums of dz [N], all
- * contiguous; any of them may be NULL.  The residual's gradient is dy. */
+ * contiguous; any of them may be NULL.  The residual's gradient is dy.  16-bit dz is rounded for the
+ * products, not for its sums.  need_dw: whether dw or dbias is going to be asked for. */
 size_t gsr_linear_backward_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N, int act,
                                          int need_dw);
 int gsr_linear_backward(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,

@@ -31,7 +31,10 @@ struct ProductArgs {
   void* out;  // gated dz: [I, 2J], gate then up
   int64_t out_row;
   float* part;      // dw: [splits][I][J]
-  float* part_sum;  // dw: [splits][I] row sums of A (the bias gradient), or NULL
+  // The bias gradient's partial sums, or NULL.  dw: [splits][I], row sums of A.  dz in 16 bits:
+  // [sum_rows][J, gated 2J], sums over a wave's rows of the gradients before they are rounded.
+  float* part_sum;
+  int64_t* sum_rows;  // dz, on the host: receives their number
   int act;
 };
 

@@ -5,19 +5,27 @@ namespace {
 
 using namespace gsr;
 
-// out[e] = sum over the splits of part[s][e] in a fixed order; the row sums follow the products.
-// 64 outputs to a workgroup, the splits shared by its four waves (a wave of few outputs alone would
-// wait for one split after the other: 33 us for 128 splits of 203 x 161, against 8).
+// out[e] = sum over s of part[s][e] in a fixed order: of `splits` weight gradients, and behind them of
+// `sum_splits` bias gradients.  64 outputs to a workgroup, the splits shared by its four waves (a wave
+// of few outputs alone would wait for one split after the other: 33 us for 128 splits of 203 x 161,
+// against 7).  With `all` rows each blockIdx.y sums `splits` of them, dw[y][e].
 template <typename T>
 __global__ __launch_bounds__(256) void reduce_kernel(const float* part, const float* part_sum,
-                                                     int splits, int64_t n, int64_t n_sum, T* dw,
-                                                     T* db) {
+                                                     int splits, int sum_splits, int64_t n,
+                                                     int64_t n_sum, int64_t all, T* dw, T* db) {
   __shared__ float sums[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t e = (int64_t)blockIdx.x * 64 + lane;
   const bool first = e < n, in = first || e - n < n_sum;
   const float* src = first ? part + e : part_sum + (in ? e - n : 0);
   const int64_t step = first ? n : n_sum;
+  if (!first) splits = sum_splits;
+  if (all) {
+    const int64_t row = (int64_t)blockIdx.y * splits;
+    src += row * step;
+    dw += (int64_t)blockIdx.y * n;
+    splits = all - row < splits ? (int)(all - row) : splits;
+  }
   const int each = (splits + 3) / 4, begin = wave * each;
   const int end = begin + each < splits ? begin + each : splits;
   float v = 0.0f;
@@ -70,29 +78,76 @@ bool x_ok(int64_t M, int64_t K, int64_t x_row, int64_t x_col) {
   return (x_col == 1 && (x_row >= K || M <= 1)) || (x_row == 1 && (x_col >= M || K == 1));
 }
 
-// The weight gradients: partial products over ranges of x's rows, then their sum.
+// The bias gradient's partial sums that a 16-bit dz kernel makes: `rows` of them of `width` at most (a
+// wave has 16 rows or more, a workgroup up to 256).  kSumGroup at a time are summed first, if there
+// are more, while the scratch they lie in is still theirs.
+constexpr int kSumGroup = 128;
+struct ColumnSums {
+  int64_t width, rows;
+  ColumnSums(int64_t M, int64_t width) : width(width), rows(up(M, 256) / 16) {}
+  bool grouped() const { return rows > kSumGroup; }
+  int64_t kept_bytes() const { return up((grouped() ? (rows + kSumGroup - 1) / kSumGroup : rows) * width * 4, 256); }
+  int64_t bytes() const { return grouped() ? up(rows * width * 4, 256) : 0; }
+};
+
+// The gradients before the activation, to `dz`, and if they are 16-bit their sums over the rows, to
+// what is returned in `sums`; `scratch` moves on behind what is kept.
+template <typename T>
+int activation_gradients(ProductArgs p, bool gated, bool need_db, char*& scratch, const float** sums,
+                         int64_t* sum_rows, hipStream_t stream) {
+  const int64_t width = gated ? 2 * p.J : p.J;
+  p.out = scratch; p.out_row = width;
+  scratch += up(p.I * width * sizeof(T), 256);
+  *sums = nullptr;
+  if (sizeof(T) == 4 || !need_db) return product_dz<T>(p, gated, scratch, stream);
+  const ColumnSums c(p.I, width);
+  float* kept = (float*)scratch;
+  scratch += c.kept_bytes();
+  p.part_sum = c.grouped() ? (float*)scratch : kept;
+  p.sum_rows = sum_rows;
+  *sums = kept;
+  if (int rc = product_dz<T>(p, gated, scratch + c.bytes(), stream)) return rc;
+  if (!c.grouped()) return 0;
+  const int64_t all = *sum_rows;
+  *sum_rows = (all + kSumGroup - 1) / kSumGroup;
+  for (int64_t at = 0; at < *sum_rows; at += 65535) {  // groups are the grid's y
+    const int64_t n = *sum_rows - at < 65535 ? *sum_rows - at : 65535, row = at * kSumGroup;
+    hipLaunchKernelGGL(reduce_kernel<float>, dim3((uint32_t)((width + 63) / 64), (uint32_t)n), dim3(256), 0, stream,
+                       p.part_sum + row * width, nullptr, kSumGroup, 0, width, 0, all - row, kept + at * width,
+                       nullptr);
+  }
+  return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+
+// The weight gradients: partial products over ranges of x's rows, then their sum.  The bias gradient
+// is dz's sum beside them, or that of `sum_rows` rows of `sums`.
 template <typename T>
 int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64_t I, const void* x,
-                     int64_t x_row, int64_t x_col, void* dw, void* db, char* scratch,
-                     hipStream_t stream) {
+                     int64_t x_row, int64_t x_col, void* dw, void* db, const float* sums, int64_t sum_rows,
+                     char* scratch, hipStream_t stream) {
   if (M == 0) {
     if (dw) hipLaunchKernelGGL(zero_kernel<T>, dim3((I * K + 255) / 256), dim3(256), 0, stream, (T*)dw, I * K);
     if (db) hipLaunchKernelGGL(zero_kernel<T>, dim3((I + 255) / 256), dim3(256), 0, stream, (T*)db, I);
     return hipGetLastError() == hipSuccess ? 0 : 2;
   }
   ProductArgs p{};
-  p.a = dz; p.a_i = 1; p.a_r = dz_row;
-  p.b[0] = x; p.b_j = x_col; p.b_r = x_row;
-  p.I = I; p.J = K; p.R = M; p.segments = 1;
-  const Ranges ranges = ranges_of(I, K, M, product_dw_huge<T>(p));
-  const int64_t splits = ranges.count;
-  p.r_chunk = ranges.rows;
-  p.part = (float*)scratch;
-  p.part_sum = db ? p.part + splits * I * K : nullptr;
-  if (int rc = product_dw<T>(p, splits, stream)) return rc;
-  const int64_t n = dw ? I * K : 0, n_sum = db ? I : 0;
-  hipLaunchKernelGGL(reduce_kernel<T>, dim3((uint32_t)((n + n_sum + 63) / 64)), dim3(256), 0, stream,
-                     p.part, p.part_sum, (int)splits, n, n_sum, (T*)dw, (T*)db);
+  if (dw || !sums) {
+    p.a = dz; p.a_i = 1; p.a_r = dz_row;
+    p.b[0] = x; p.b_j = x_col; p.b_r = x_row;
+    p.I = I; p.J = K; p.R = M; p.segments = 1;
+    const Ranges ranges = ranges_of(I, K, M, product_dw_huge<T>(p));
+    p.r_chunk = ranges.rows;
+    p.part = (float*)scratch;
+    p.part_sum = db && !sums ? p.part + ranges.count * I * K : nullptr;
+    if (int rc = product_dw<T>(p, ranges.count, stream)) return rc;
+    if (!sums) sums = p.part_sum, sum_rows = ranges.count;
+    const int64_t n = dw ? I * K : 0, n_sum = db ? I : 0;
+    hipLaunchKernelGGL(reduce_kernel<T>, dim3((uint32_t)((n + n_sum + 63) / 64)), dim3(256), 0, stream, p.part, sums,
+                       (int)ranges.count, (int)sum_rows, n, n_sum, 0, (T*)dw, (T*)db);
+  } else {
+    hipLaunchKernelGGL(reduce_kernel<T>, dim3((uint32_t)((I + 63) / 64)), dim3(256), 0, stream, nullptr, sums, 0,
+                       (int)sum_rows, 0, I, 0, nullptr, (T*)db);
+  }
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
@@ -103,19 +158,22 @@ size_t partial_bytes(int64_t M, int64_t K, int64_t I) {
   return (size_t)n * I * (K + 1) * 4;
 }
 
-// Scratch of a backward, in order: the pre-activation gradients, then what one product at a time
-// needs (the weights' images, the partial sums).
+// Scratch of a backward, in order: the gradients before the activation, their sums, then what one
+// product at a time needs (the weights' images, the partial sums).
 template <typename T>
 size_t backward_bytes(int64_t M, int64_t K, int64_t N, bool gated, bool has_dz, bool need_dw) {
   const int64_t width = gated ? 2 * N : N;
+  const bool column_sums = has_dz && need_dw && sizeof(T) == 2;
+  const ColumnSums c(M, width);
   size_t most = has_dz ? product_scratch<T>(M, N, K, gated) : 0;
+  if (column_sums) most += c.bytes();
   if (!gated) {
     const size_t dx = product_scratch<T>(M, K, N, false);
     most = dx > most ? dx : most;
   }
   const size_t dw = need_dw ? partial_bytes(M, K, width) : 0;
   most = dw > most ? dw : most;
-  return (has_dz ? (size_t)up(M * width * sizeof(T), 256) : 0) + most;
+  return (has_dz ? (size_t)up(M * width * sizeof(T), 256) : 0) + (column_sums ? c.kept_bytes() : 0) + most;
 }
 
 template <typename T>
@@ -123,14 +181,13 @@ int linear_backward(const ProductArgs& fwd, const void* dy, int64_t dy_row, void
                     void* db, char* scratch, hipStream_t stream) {
   const int64_t M = fwd.I, K = fwd.R, N = fwd.J;
   const void* dz = dy;
-  int64_t dz_row = dy_row;
+  int64_t dz_row = dy_row, sum_rows = 0;
+  const float* sums = nullptr;
   if (fwd.act != GSR_ACT_NONE && M > 0) {
     ProductArgs p = fwd;
     p.extra = dy; p.extra_row = dy_row;
-    p.out = scratch; p.out_row = N;
     dz = scratch; dz_row = N;
-    scratch += up(M * N * sizeof(T), 256);
-    if (int rc = product_dz<T>(p, false, scratch, stream)) return rc;
+    if (int rc = activation_gradients<T>(p, false, db, scratch, &sums, &sum_rows, stream)) return rc;
   }
   if (dx && M > 0) {
     ProductArgs p{};
@@ -141,7 +198,7 @@ int linear_backward(const ProductArgs& fwd, const void* dy, int64_t dy_row, void
     if (int rc = product_dx<T>(p, scratch, stream)) return rc;
   }
   if (!dw && !db) return 0;
-  return weight_gradients<T>(dz, dz_row, M, K, N, fwd.a, fwd.a_i, fwd.a_r, dw, db, scratch, stream);
+  return weight_gradients<T>(dz, dz_row, M, K, N, fwd.a, fwd.a_i, fwd.a_r, dw, db, sums, sum_rows, scratch, stream);
 }
 
 template <typename T>
@@ -149,12 +206,12 @@ int gated_backward(const ProductArgs& fwd, const void* dh, int64_t dh_row, void*
                    void* db, char* scratch, hipStream_t stream) {
   const int64_t M = fwd.I, K = fwd.R, N = fwd.J;
   const void* dz = scratch;
+  int64_t sum_rows = 0;
+  const float* sums = nullptr;
   if (M > 0) {
     ProductArgs p = fwd;
     p.extra = dh; p.extra_row = dh_row;
-    p.out = scratch; p.out_row = 2 * N;
-    scratch += up(2 * M * N * sizeof(T), 256);
-    if (int rc = product_dz<T>(p, true, scratch, stream)) return rc;
+    if (int rc = activation_gradients<T>(p, true, db, scratch, &sums, &sum_rows, stream)) return rc;
     if (dx) {
       ProductArgs q{};
       q.a = dz; q.a_i = 2 * N; q.a_r = 1;
@@ -165,7 +222,7 @@ int gated_backward(const ProductArgs& fwd, const void* dh, int64_t dh_row, void*
     }
   }
   if (!dw && !db) return 0;
-  return weight_gradients<T>(dz, 2 * N, M, K, 2 * N, fwd.a, fwd.a_i, 1, dw, db, scratch, stream);
+  return weight_gradients<T>(dz, 2 * N, M, K, 2 * N, fwd.a, fwd.a_i, 1, dw, db, sums, sum_rows, scratch, stream);
 }
 
 ProductArgs forward_args(int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,

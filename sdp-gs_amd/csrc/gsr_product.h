@@ -410,6 +410,29 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, int64_t i, int64_
   if (EPI == EPI_DZ && GATED) store_run<T, RUN>(out + p.J, w, n);
 }
 
+// Whether a dz kernel also makes the bias gradient's partial sums: with 16-bit results, whose
+// rounding would be in every sum of them (an error as large as that of the sum's own rounding).  A
+// sum of 32-bit results loses nothing, it is made beside the weight gradients.
+template <typename T, int EPI> constexpr bool kColumnSums = EPI == EPI_DZ && sizeof(T) == 2;
+
+// v[k] summed over the 16 lanes of a DPP row, n of them stored by the first.
+template <int RUN>
+__device__ __forceinline__ void store_sums(float* p, int m, int64_t n, float (&v)[RUN]) {
+  auto ror = [](auto by, float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + decltype(by)::value, 15, 15, false));
+  };
+#pragma unroll
+  for (int k = 0; k < RUN; k++) {
+    v[k] += ror(Const<8>(), v[k]);
+    v[k] += ror(Const<4>(), v[k]);
+    v[k] += ror(Const<2>(), v[k]);
+    v[k] += ror(Const<1>(), v[k]);
+  }
+  if (m) return;
+#pragma unroll
+  for (int h = 0; h < RUN; h += 4) store_run<float, 4>(p + h, {v[h], v[h + 1], v[h + 2], v[h + 3]}, n - h);
+}
+
 // f(integral constant of the activation): one branch for a whole epilogue.
 template <int EPI, typename F>
 __device__ __forceinline__ void with_act(int act, F f) {
@@ -428,7 +451,7 @@ __device__ __noinline__ float exact_sum(const float* a, int64_t a_i, int64_t a_r
   for (int s = 0; s < segments; s++) {
     const float* A = a + s * a_segment + i * a_i;
     const float* B = (s ? b1 : b0) + j * b_j;
-    for (int64_t r = r0; r < r1; r++) v = fmaf(A[r * a_r], b0 ? B[r * b_r] : 1.0f, v);
+    for (int64_t r = r0; r < r1 && v == v; r++) v = fmaf(A[r * a_r], b0 ? B[r * b_r] : 1.0f, v);  // NaN stays
   }
   return v;
 }
@@ -639,6 +662,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
         if (p.bias[0]) load_run<T, RUN>(bias, (const T*)p.bias[0] + j, n);
         if (GATED && p.bias[1]) load_run<T, RUN>(bias1, (const T*)p.bias[1] + j, n);
       }
+      float total[RUN] = {}, total1[RUN] = {};
 #pragma unroll
       for (int u = 0; u < NI; u++) {
         const int64_t i = i0 + (wi * NI + u) * 16 + m;
@@ -655,6 +679,18 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
           if (EPI != EPI_PLAIN && p.extra) load_run<T, RUN>(ex, (const T*)p.extra + i * p.extra_row + j, n);
           epilogue<T, EPI, GATED, true, decltype(act)::value, RUN>(p, i, j, n, v, w, ex);
         }
+        if (kColumnSums<T, EPI>) {
+#pragma unroll
+          for (int k = 0; k < RUN; k++) {
+            total[k] += v[k];
+            if (GATED) total1[k] += w[k];
+          }
+        }
+      }
+      if (kColumnSums<T, EPI> && p.part_sum) {
+        float* sums_of = p.part_sum + (at.i * WI + wi) * (GATED ? 2 * p.J : p.J) + j;
+        store_sums(sums_of, m, n, total);
+        if (GATED) store_sums(sums_of + p.J, m, n, total1);
       }
     }
   });
@@ -677,6 +713,7 @@ int launch_tiles(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   const int64_t ti = (p.I + BI - 1) / BI, tj = (p.J + kOut - 1) / kOut;
   if (ti > 0x7fffffff / tj || ti * tj > 0x7ffffff0 / splits) return 1;
   const int64_t total = ti * tj * splits, grid = (total + 7) / 8 * 8;
+  if (kColumnSums<T, EPI> && p.part_sum) *p.sum_rows = ti * WI;
   hipLaunchKernelGGL((product_kernel<T, RCA, RCB, EPI, GATED, DIRECT, BI, WI, BJ, WJ>), dim3((uint32_t)grid),
                      dim3(64 * WI * WJ), 0, stream, p, (uint32_t)ti, (uint32_t)tj, (uint32_t)splits);
   return hipGetLastError() == hipSuccess ? 0 : 2;
@@ -692,9 +729,12 @@ int launch_product(const ProductArgs& p, int64_t splits, hipStream_t stream) {
 // Whether a 16-bit weight gradient of I x J takes 256 x 256 tiles (if its operands are aligned).
 inline bool takes_huge_dw(int64_t I, int64_t J) { return I > 128 && J > 128; }  // 256 x 256 tiles
 
-// The tile by the size of C: 256 x 256 where one a CU keeps it busy (operands straight to LDS),
-// 128 x 128 where there are outputs for it, 128 x 64 for narrow results, 64 x 64 where the larger
-// ones would leave CUs without work.
+// The tile by the size of C.  256 x 256 where one a CU keeps it busy and operands go straight to LDS
+// (us, these : 128 x 128; bf16 8192x4096x4096 264 : 332, weight gradients of 762048x256x512 290 : 330,
+// 100000x1024x1024 272 : 302).  128 x 128 where there is one for each CU, 64 x 64 below that (64 x 64
+// : 128 x 128; bf16 512x4096x4096 43 : 52, 2048x512x512 7.1 : 10.4, fp32 17 : 34; at 1024x4096x4096,
+// 256 tiles, bf16 55 : 55, fp32 296 : 257).  128 x 64 for up to 64 columns of many rows (fp32
+// weight gradient of 762048x64x256 271, with 64 x 64 348; but of 762048x3x64, 64 rows, 128 : 76).
 template <typename T, bool RCA, bool RCB, int EPI>
 int launch_linear(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
@@ -703,9 +743,10 @@ int launch_linear(const ProductArgs& p, int64_t splits, hipStream_t stream) {
       return launch_tiles<T, RCA, RCB, EPI, false, true, 256, 4, 256, 2>(p, splits, stream);
   }
   const int64_t large = (p.I + 127) / 128 * ((p.J + 127) / 128) * splits;
-  if (p.J > 64 && large >= 256) return launch_product<T, RCA, RCB, EPI, false, 128, 2, 128, 2>(p, splits, stream);
-  if (p.J <= 64 && (p.I + 127) / 128 * splits >= 256)
+  if (p.I > 64 && large >= 256) {
+    if (p.J > 64) return launch_product<T, RCA, RCB, EPI, false, 128, 2, 128, 2>(p, splits, stream);
     return launch_product<T, RCA, RCB, EPI, false, 128, 4, 64, 1>(p, splits, stream);
+  }
   return launch_product<T, RCA, RCB, EPI, false, 64, 4, 64, 1>(p, splits, stream);
 }
 

@@ -218,6 +218,7 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
         for (int s = 0; s < kRuns; s++) {
           const int64_t j = j0 + column_of(s), n = FULL ? RUN : p.J - j;
           if (!FULL && n <= 0) continue;
+          float total[RUN] = {}, total1[RUN] = {};
 #pragma unroll
           for (int u = 0; u < NI; u++) {
             const int64_t i = i0 + u * 16 + m;
@@ -230,10 +231,22 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
               if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4];
             }
             epilogue<T, EPI, GATED, EXTRA, decltype(act)::value, RUN>(p, i, j, n, v, w, e);
+            if (kColumnSums<T, EPI>) {
+#pragma unroll
+              for (int k = 0; k < RUN; k++) {
+                total[k] += v[k];
+                if (GATED) total1[k] += w[k];
+              }
+            }
+          }
+          if (kColumnSums<T, EPI> && p.part_sum) {
+            float* sums = p.part_sum + ((int64_t)(id / parts) * kWaves + wave) * (GATED ? 2 * p.J : p.J) + j;
+            store_sums(sums, m, n, total);
+            if (GATED) store_sums(sums + p.J, m, n, total1);
           }
         }
         // This wave's part of the next image has to be there.  It was asked for before the stores of
-        // this tile, which may go on.
+        // this tile, the last kStores of which may go on.
         constexpr int kStores = NI * kRuns * (EPI == EPI_DZ && GATED ? 2 : 1);
         if (FULL) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -277,6 +290,7 @@ int launch_strip(const ProductArgs& p, char* scratch, hipStream_t stream) {
   parts = (tiles + part_tiles - 1) / part_tiles;
   const int64_t items = strips * parts;
   if (items > 0x7ffffff0 || chunks > 0x7fffffff) return 1;
+  if (kColumnSums<T, EPI> && p.part_sum) *p.sum_rows = strips * S::kWaves;
   // one small tile of weights is made by every workgroup itself: cheaper than a launch before this
   // one (762048x3x64 in 32 bits: 67 us a call with it, 57 without); not a large one (bf16
   // 762048x256x64: 101 us with it, 142 without)
@@ -319,7 +333,7 @@ template <typename T, int EPI>
 int forward_or_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) {
   const bool strips = takes_strips(p.I, p.R);
   if constexpr (EPI == EPI_FORWARD)
-    if (takes_rows(p)) return gated ? launch_rows<T, EPI, true>(p, s) : launch_rows<T, EPI, false>(p, s);
+    if (takes_rows<T>(p, gated)) return gated ? launch_rows<T, EPI, true>(p, s) : launch_rows<T, EPI, false>(p, s);
   if (gated) return strips ? launch_strips<T, true, EPI, true>(p, scratch, s) : launch_gated<T, EPI>(p, s);
   if (p.a_r == 1)
     return strips ? launch_strips<T, true, EPI, false>(p, scratch, s) : launch_linear<T, true, true, EPI>(p, 1, s);

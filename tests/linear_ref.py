@@ -8,7 +8,9 @@ Bounds, per element, from the arithmetic alone (u = half a step of the result's 
     erf to 1.5e-7, exp and reciprocal to a few 2^-24, together below |z| 2^-21
   * its slope: the curvature (at most 0.8) times the argument's error, and 2^-20 (1 + |z|); relu's
     jumps where z is within its error of 0
-  * each rounding to the type: u |value|; for float16 also half its smallest step, 2^-25
+  * each rounding to the type: u |value|; for float16 also half its smallest step, 2^-25.  The
+    gradients before the activation are rounded for the products that follow, but not for the
+    bias gradients, which are their sums.
 """
 import torch
 
@@ -62,17 +64,20 @@ def product(x, w, b):
     return z, e
 
 
-def gradients(dz, edz, x, ws, t):
+def gradients(dz, edz, x, ws, t, round_dz=True):
     """{name: (value, bound)} of dx, and each weight's and bias's gradient, from the pre-activation
-    gradients dz[i] of products x w_i^T."""
+    gradients dz[i] of products x w_i^T, within edz[i] before they are rounded."""
     M, N = dz[0].shape
+    eb = edz
+    if round_dz:
+        edz = [e + rounded(d, t) for d, e in zip(dz, edz)]
     dx = sum(d @ w for d, w in zip(dz, ws))
     ex = sum(e @ w.abs() + sum_error(2 * N, d, w) for d, e, w in zip(dz, edz, ws))
     out = {"x": (dx, ex + rounded(dx, t))}
-    for i, (d, e) in enumerate(zip(dz, edz)):
+    for i, (d, e, f) in enumerate(zip(dz, edz, eb)):
         dw, db = d.t() @ x, d.sum(0)
         out[f"w{i}"] = (dw, e.t() @ x.abs() + sum_error(M, d.t(), x) + rounded(dw, t))
-        out[f"b{i}"] = (db, e.sum(0) + (M + 10) * 2.0 ** -24 * d.abs().sum(0) + rounded(db, t))
+        out[f"b{i}"] = (db, f.sum(0) + (M + 10) * 2.0 ** -24 * d.abs().sum(0) + rounded(db, t))
     return out
 
 
@@ -86,8 +91,8 @@ def linear(x, w, b, r, kind, t, dy=None):
         dz = dy * act_slope(z, kind)
         edz = dy.abs() * slope_error(z, ez, kind)
         if kind != "none":
-            edz = edz + 2.0 ** -23 * dz.abs() + rounded(dz, t)
-        out.update(gradients([dz], [edz], x, [w], t))
+            edz = edz + 2.0 ** -23 * dz.abs()
+        out.update(gradients([dz], [edz], x, [w], t, kind != "none"))
     return out
 
 
@@ -102,7 +107,7 @@ def gated(x, wg, wu, bg, bu, kind, t, dh=None):
         dg, du = dh * u * s, dh * a
         edg = dh.abs() * (es * u.abs() + eu * s.abs() + es * eu) + 2.0 ** -22 * dg.abs()
         edu = dh.abs() * ea + 2.0 ** -23 * du.abs()
-        out.update(gradients([dg, du], [edg + rounded(dg, t), edu + rounded(du, t)], x, [wg, wu], t))
+        out.update(gradients([dg, du], [edg, edu], x, [wg, wu], t))
     return out
 
 

@@ -49,7 +49,13 @@ SIZES = [(1, 1, 1), (1, 512, 512), (2, 3, 5), (5, 4096, 33), (17, 129, 1000), (3
          (300, 7, 1), (512, 1, 16), (777, 161, 203), (2049, 96, 40), (3000, 33, 130), (4100, 31, 70), (5000, 100, 129),
          # enough rows for the kernel that keeps its rows: 1, 2, 4, 6 and 8 steps of 32 inputs
          (32769, 31, 70), (32800, 3, 64), (33000, 63, 33), (32768, 128, 64), (32771, 161, 203),
-         (32900, 256, 130), (33001, 250, 40)]
+         (32900, 256, 130), (33001, 250, 40),
+         # the largest tiles, operands straight to LDS, the last step of either sum ragged; the same
+         # sizes where nothing is aligned; a narrow weight gradient
+         (33001, 264, 264), (16500, 72, 1032), (33001, 263, 265), (20000, 40, 200),
+         # around the sizes where few rows end
+         (32, 520, 640), (33, 520, 640), (63, 520, 640), (66, 520, 640), (129, 520, 640),
+         (256, 520, 640), (257, 520, 640)]
 
 
 @gpu
@@ -232,6 +238,27 @@ def test_rows_beyond_the_last_are_untouched():
             assert rc == 0
             ref.check({"y": y[:M, :N]}, _want(d, "relu", grads=False))
             assert bool((y[M:] == 7).all()) and bool((y[:, N:] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N", [(8_400_000, 256, 256), (4_200_000, 512, 512)])
+def test_more_than_2_to_31_elements(M, K, N):
+    """Offsets of operands and results pass 32 bits.  Only the first and the last rows have a gradient
+    that is not zero, so these rows' formulas give all gradients."""
+    t, n = torch.bfloat16, 300
+    d = ref.inputs(15, 2 * n, K, N, t, "cuda")
+    ends = {k: d[k] for k in ("x", "dy")}
+    for k, v in ends.items():
+        big = torch.zeros(M, v.shape[1], dtype=t, device="cuda")
+        big[:n], big[-n:] = v[:n], v[n:]
+        d[k] = big
+    got = _run(d, "silu")
+    for k in ("y", "x"):
+        got[k] = torch.cat([got[k][:n], got[k][-n:]])
+    e = {**d, **ends}
+    want = _want(e, "silu")
+    # sums over M rows, all but 2 n of them zero: exact zeros add nothing
+    ref.check(got, want)
 
 
 @gpu
