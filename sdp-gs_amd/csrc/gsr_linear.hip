@@ -79,12 +79,13 @@ bool x_ok(int64_t M, int64_t K, int64_t x_row, int64_t x_col) {
 }
 
 // The bias gradient's partial sums that a 16-bit dz kernel makes: `rows` of them of `width` at most (a
-// wave has 16 rows or more, a workgroup up to 256).  kSumGroup at a time are summed first, if there
+// wave has 16 rows or more, a workgroup up to 256; four rows where the product is cut, which more than
+// 8192 are not).  kSumGroup at a time are summed first, if there
 // are more, while the scratch they lie in is still theirs.
 constexpr int kSumGroup = 128;
 struct ColumnSums {
   int64_t width, rows;
-  ColumnSums(int64_t M, int64_t width) : width(width), rows(up(M, 256) / 16) {}
+  ColumnSums(int64_t M, int64_t width) : width(width), rows(up(M, 256) / (M <= 8192 ? 4 : 16)) {}
   bool grouped() const { return rows > kSumGroup; }
   int64_t kept_bytes() const { return up((grouped() ? (rows + kSumGroup - 1) / kSumGroup : rows) * width * 4, 256); }
   int64_t bytes() const { return grouped() ? up(rows * width * 4, 256) : 0; }
@@ -165,12 +166,10 @@ size_t backward_bytes(int64_t M, int64_t K, int64_t N, bool gated, bool has_dz, 
   const int64_t width = gated ? 2 * N : N;
   const bool column_sums = has_dz && need_dw && sizeof(T) == 2;
   const ColumnSums c(M, width);
-  size_t most = has_dz ? product_scratch<T>(M, N, K, gated) : 0;
+  size_t most = has_dz ? dz_scratch<T>(M, K, N, gated) : 0;
   if (column_sums) most += c.bytes();
-  if (!gated) {
-    const size_t dx = product_scratch<T>(M, K, N, false);
-    most = dx > most ? dx : most;
-  }
+  const size_t dx = dx_scratch<T>(M, K, N, gated ? 2 : 1);
+  most = dx > most ? dx : most;
   const size_t dw = need_dw ? partial_bytes(M, K, width) : 0;
   most = dw > most ? dw : most;
   return (has_dz ? (size_t)up(M * width * sizeof(T), 256) : 0) + (column_sums ? c.kept_bytes() : 0) + most;
@@ -255,7 +254,7 @@ int forward(int dtype, const ProductArgs& p, bool gated, void* scratch, void* st
 
 size_t forward_bytes(int dtype, int64_t M, int64_t K, int64_t N, bool gated) {
   return with_type(dtype, [&](auto t) {
-    return product_scratch<typename Pointee<decltype(t)>::type>(M, N, K, gated);
+    return forward_scratch<typename Pointee<decltype(t)>::type>(M, K, N, gated);
   });
 }
 

@@ -497,8 +497,15 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
   const int wave = threadIdx.x >> 6, wi = wave / WJ, wj = wave % WJ;
   const int64_t i0 = at.i * BI, j0 = (int64_t)at.j * kOut;
   int64_t r_begin = 0, r_end = p.R;
+  const T *a0 = (const T*)p.a, *b0 = (const T*)p.b[0];
   if (EPI == EPI_PARTIAL) {
-    r_begin = (int64_t)at.split * p.r_chunk;
+    uint32_t range = at.split;
+    if (!GATED && p.segments == 2 && range >= splits / 2) {  // the second segment's ranges
+      range -= splits / 2;
+      a0 += p.a_segment;
+      b0 = (const T*)p.b[1];
+    }
+    r_begin = (int64_t)range * p.r_chunk;
     r_end = r_begin + p.r_chunk < p.R ? r_begin + p.r_chunk : p.R;
   }
   const int64_t lda = RCA ? p.a_i : p.a_r, ldb = RCB ? p.b_j : p.b_r;
@@ -509,8 +516,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
   constexpr int kSplit = GATED ? BJ / 2 : 0;
   // Where step `it` starts: f(A, B, r0).
   auto at_step = [&](uint32_t it, auto f) {
-    const T* a = (const T*)p.a;
-    const T* b = (const T*)p.b[0];
+    const T *a = a0, *b = b0;
     if (EPI == EPI_PLAIN && it >= steps) {  // the second segment
       it -= steps;
       a += p.a_segment;
@@ -633,7 +639,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
             const bool second = GATED && row >= kOut;
             const int64_t j = j0 + (second ? row - kOut : row);
             if (j < p.J && !(fabsf(acc[u][t][v]) <= 3.4e38f))
-              acc[u][t][v] = exact_sum((const float*)p.a, p.a_i, p.a_r, (const float*)p.b[second ? 1 : 0],
+              acc[u][t][v] = exact_sum((const float*)a0, p.a_i, p.a_r, second ? (const float*)p.b[1] : (const float*)b0,
                                        (const float*)p.b[1], p.b_j, p.b_r, segments, p.a_segment, i, j,
                                        r_begin, r_end);
           }
@@ -674,7 +680,9 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
           if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4] + bias1[k];
         }
         if constexpr (EPI == EPI_PARTIAL) {
-          store_run<float, RUN>(p.part + ((int64_t)at.split * p.I + i) * p.J + j, v, n);
+          float* part = p.part + ((int64_t)at.split * p.I + i) * (GATED ? 2 * p.J : p.J) + j;
+          store_run<float, RUN>(part, v, n);
+          if (GATED) store_run<float, RUN>(part + p.J, w, n);
         } else {
           if (EPI != EPI_PLAIN && p.extra) load_run<T, RUN>(ex, (const T*)p.extra + i * p.extra_row + j, n);
           epilogue<T, EPI, GATED, true, decltype(act)::value, RUN>(p, i, j, n, v, w, ex);
@@ -757,8 +765,113 @@ int launch_gated(const ProductArgs& p, hipStream_t stream) {
   return launch_product<T, true, true, EPI, true, 64, 4, 128, 1>(p, 1, stream);
 }
 
+// Few tiles and a long sum: the sum is cut into ranges, so that there is work for every CU, and a
+// second kernel adds the ranges (in their order: the same bits every time) and has the epilogue.
+// Ranges per segment for C of I x J, summed over R of each of `segments`; 1: not cut.  us, cut :
+// whole, fp32 300x4096x512 24 : 105, 512x1024x1024 21 : 30, 4096x512x128 14.8 : 16.7; bf16
+// 300x4096x512 12.8 : 35.7, 128x2048x2048 12.2 : 15.7, but 512x1024x1024 13.8 : 9.7, 4096x512x128
+// 10 : 6.9 (a step of 16-bit operands takes less time, the second kernel as long).
+template <typename T>
+int64_t cuts_of(int64_t I, int64_t J, int64_t R, int64_t segments) {
+  const int64_t tiles = (I + 63) / 64 * ((J + 63) / 64) * segments;
+  if (tiles > 128 || R < (sizeof(T) == 4 ? 512 : 2048)) return 1;
+  const int64_t most = R / 256, want = 512 / tiles;
+  return want < most ? want : most;
+}
+inline int64_t cut_rows(int64_t R, int64_t cuts) { return ((R + cuts - 1) / cuts + 63) / 64 * 64; }
+template <typename T>
+size_t cut_bytes(int64_t I, int64_t J, int64_t R, int64_t segments, bool gated) {
+  const int64_t cuts = cuts_of<T>(I, J, R, segments);
+  return cuts > 1 ? (size_t)cuts * segments * I * J * (gated ? 8 : 4) : 0;
+}
+
+// A wave has one row of 64 columns, a workgroup four.
+template <typename T, int EPI, bool GATED>
+__global__ __launch_bounds__(256) void finish_kernel(ProductArgs p, uint32_t splits) {
+  __shared__ float rows[GATED ? 2 : 1][4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t j = (int64_t)blockIdx.x * 64 + lane, i = (int64_t)blockIdx.y * 4 + wave;
+  const bool in = i < p.I && j < p.J;
+  const int64_t width = GATED ? 2 * p.J : p.J, step = p.I * width;
+  float v = 0.0f, w = 0.0f;
+  if (in) {
+    const float* part = p.part + i * width + j;
+    uint32_t s = 0;
+    for (; s + 8 <= splits; s += 8) {
+      float x[8], y[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        x[k] = part[(s + k) * step];
+        if (GATED) y[k] = part[(s + k) * step + p.J];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        v += x[k];
+        if (GATED) w += y[k];
+      }
+    }
+    for (; s < splits; s++) {
+      v += part[s * step];
+      if (GATED) w += part[s * step + p.J];
+    }
+    if (EPI != EPI_PLAIN) {
+      if (p.bias[0]) v += to_f(((const T*)p.bias[0])[j]);
+      if (GATED && p.bias[1]) w += to_f(((const T*)p.bias[1])[j]);
+    }
+    const float e = EPI != EPI_PLAIN && p.extra ? to_f(((const T*)p.extra)[i * p.extra_row + j]) : 0.0f;
+    with_act<EPI>(p.act, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      if (EPI == EPI_FORWARD) {
+        v = act_value<ACT>(v);
+        if (GATED) v *= w;
+        if (p.extra) v += e;
+      } else if (EPI == EPI_DZ) {
+        float a;
+        const float slope = act_both<ACT>(v, a);
+        v = GATED ? e * w * slope : e * slope;
+        if (GATED) w = e * a;
+      }
+    });
+    T* out = (T*)p.out + i * p.out_row + j;
+    out[0] = from_f<T>(v);
+    if (EPI == EPI_DZ && GATED) out[p.J] = from_f<T>(w);
+  }
+  if (kColumnSums<T, EPI> && p.part_sum) {
+    rows[0][wave][lane] = v;
+    if (GATED) rows[GATED][wave][lane] = w;
+    __syncthreads();
+    if (wave || j >= p.J) return;
+    float* sums = p.part_sum + blockIdx.y * width + j;
+#pragma unroll
+    for (int h = 0; h < (GATED ? 2 : 1); h++)
+      sums[h * p.J] = rows[h][0][lane] + rows[h][1][lane] + rows[h][2][lane] + rows[h][3][lane];
+  }
+}
+
+// The product cut into `cuts` ranges per segment, their results in `scratch`.
+template <typename T, bool RCB, int EPI, bool GATED>
+int launch_cut(ProductArgs p, int64_t cuts, char* scratch, hipStream_t stream) {
+  p.r_chunk = cut_rows(p.R, cuts);
+  const int64_t splits = (p.R + p.r_chunk - 1) / p.r_chunk * p.segments;
+  p.part = (float*)scratch;
+  float* sums = p.part_sum;
+  p.part_sum = nullptr;
+  const int rc = GATED ? launch_product<T, true, RCB, EPI_PARTIAL, GATED, 64, 4, 128, 1>(p, splits, stream)
+                       : launch_product<T, true, RCB, EPI_PARTIAL, GATED, 64, 4, 64, 1>(p, splits, stream);
+  if (rc) return rc;
+  p.part_sum = sums;
+  const int64_t rows = (p.I + 3) / 4;
+  if (kColumnSums<T, EPI> && sums) *p.sum_rows = rows;
+  hipLaunchKernelGGL((finish_kernel<T, EPI, GATED>), dim3((uint32_t)((p.J + 63) / 64), (uint32_t)rows), dim3(256), 0,
+                     stream, p, (uint32_t)splits);
+  return hipGetLastError() == hipSuccess ? 0 : 2;
+}
+
 // What gsr_linear.hip needs of each type (gsr_linear_f32.hip, _f16.hip, _bf16.hip).
-template <typename T> size_t product_scratch(int64_t I, int64_t J, int64_t R, bool gated);
+// Scratch of a forward, dz or dx product of these sizes; dx is over `segments`.
+template <typename T> size_t forward_scratch(int64_t M, int64_t K, int64_t N, bool gated);
+template <typename T> size_t dz_scratch(int64_t M, int64_t K, int64_t N, bool gated);
+template <typename T> size_t dx_scratch(int64_t M, int64_t K, int64_t N, int segments);
 template <typename T> int product_forward(const ProductArgs& p, bool gated, char* scratch, hipStream_t s);
 template <typename T> int product_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s);
 template <typename T> int product_dx(const ProductArgs& p, char* scratch, hipStream_t s);

@@ -129,11 +129,11 @@ int launch_rows(const ProductArgs& p, hipStream_t s) {
 // 32x1024x6144 (96) 8.2 : 9.1, gated 16x2048x5504 17 : 22, 64x2048x5504 28 : 23; fp32
 // 128x4096x4096 (128) 84 : 104, 128x1024x6144 (192) 35 : 30, 64x1024x6144 (96) 24 : 28.
 template <typename T>
-bool takes_rows(const ProductArgs& p, bool gated) {
-  if (p.a_r != 1 || p.I > 256) return false;
-  const int64_t tiles = (p.I + 63) / 64 * ((p.J + 63) / 64);
-  if (sizeof(T) == 4) return p.I <= 64 || tiles <= 128;
-  return p.I <= 32 || (p.I <= 64 && tiles <= 64 && !gated);
+bool rows_sizes(int64_t I, int64_t J, bool gated) {
+  if (I > 256) return false;
+  const int64_t tiles = (I + 63) / 64 * ((J + 63) / 64);
+  if (sizeof(T) == 4) return I <= 64 || tiles <= 128;
+  return I <= 32 || (I <= 64 && tiles <= 64 && !gated);
 }
 
 }  // namespace gsr

@@ -329,24 +329,52 @@ int launch_strips(const ProductArgs& p, char* scratch, hipStream_t s) {
   return with_steps(p.R, [&](auto ks) { return launch_strip<T, RCA, EPI, GATED, decltype(ks)::value>(p, scratch, s); });
 }
 
+template <typename T>
+size_t strips_scratch(int64_t J, int64_t R, bool gated) {
+  return with_steps(R, [&](auto ks) {
+    constexpr int KS = decltype(ks)::value;
+    return gated ? image_bytes<T, true, KS>(J) : image_bytes<T, false, KS>(J);
+  });
+}
+
+template <typename T, int EPI>
+size_t forward_or_dz_scratch(int64_t M, int64_t K, int64_t N, bool gated) {
+  if (takes_strips(M, K)) return strips_scratch<T>(N, K, gated);
+  return EPI == EPI_FORWARD && rows_sizes<T>(M, N, gated) ? 0 : cut_bytes<T>(M, N, K, 1, gated);
+}
+
 template <typename T, int EPI>
 int forward_or_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) {
-  const bool strips = takes_strips(p.I, p.R);
+  const bool strips = takes_strips(p.I, p.R), few = EPI == EPI_FORWARD && rows_sizes<T>(p.I, p.J, gated);
   if constexpr (EPI == EPI_FORWARD)
-    if (takes_rows<T>(p, gated)) return gated ? launch_rows<T, EPI, true>(p, s) : launch_rows<T, EPI, false>(p, s);
+    if (few && p.a_r == 1) return gated ? launch_rows<T, EPI, true>(p, s) : launch_rows<T, EPI, false>(p, s);
+  const int64_t cuts = strips || few || p.a_r != 1 ? 1 : cuts_of<T>(p.I, p.J, p.R, 1);
+  if (cuts > 1)
+    return gated ? launch_cut<T, true, EPI, true>(p, cuts, scratch, s) : launch_cut<T, true, EPI, false>(p, cuts, scratch, s);
   if (gated) return strips ? launch_strips<T, true, EPI, true>(p, scratch, s) : launch_gated<T, EPI>(p, s);
   if (p.a_r == 1)
     return strips ? launch_strips<T, true, EPI, false>(p, scratch, s) : launch_linear<T, true, true, EPI>(p, 1, s);
   return strips ? launch_strips<T, false, EPI, false>(p, scratch, s) : launch_linear<T, false, true, EPI>(p, 1, s);
 }
 
+template <typename T>
+int dx_product(const ProductArgs& p, char* scratch, hipStream_t s) {
+  if (p.segments == 1 && takes_strips(p.I, p.R)) return launch_strips<T, true, EPI_PLAIN, false>(p, scratch, s);
+  const int64_t cuts = cuts_of<T>(p.I, p.J, p.R, p.segments);
+  if (cuts > 1) return launch_cut<T, false, EPI_PLAIN, false>(p, cuts, scratch, s);
+  return launch_linear<T, true, false, EPI_PLAIN>(p, 1, s);
+}
+
 #define GSR_PRODUCTS(T)                                                                              \
-  template <> size_t product_scratch<T>(int64_t I, int64_t J, int64_t R, bool gated) {               \
-    if (!takes_strips(I, R)) return 0;                                                               \
-    return with_steps(R, [&](auto ks) {                                                              \
-      constexpr int KS = decltype(ks)::value;                                                        \
-      return gated ? image_bytes<T, true, KS>(J) : image_bytes<T, false, KS>(J);                     \
-    });                                                                                              \
+  template <> size_t forward_scratch<T>(int64_t M, int64_t K, int64_t N, bool gated) {               \
+    return forward_or_dz_scratch<T, EPI_FORWARD>(M, K, N, gated);                                    \
+  }                                                                                                  \
+  template <> size_t dz_scratch<T>(int64_t M, int64_t K, int64_t N, bool gated) {                    \
+    return forward_or_dz_scratch<T, EPI_DZ>(M, K, N, gated);                                         \
+  }                                                                                                  \
+  template <> size_t dx_scratch<T>(int64_t M, int64_t K, int64_t N, int segments) {                  \
+    if (segments == 1 && takes_strips(M, N)) return strips_scratch<T>(K, N, false);                  \
+    return cut_bytes<T>(M, K, N, segments, false);                                                      \
   }                                                                                                  \
   template <> int product_forward<T>(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) { \
     return forward_or_dz<T, EPI_FORWARD>(p, gated, scratch, s);                                      \
@@ -355,9 +383,7 @@ int forward_or_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s
     return forward_or_dz<T, EPI_DZ>(p, gated, scratch, s);                                           \
   }                                                                                                  \
   template <> int product_dx<T>(const ProductArgs& p, char* scratch, hipStream_t s) {                \
-    if (p.segments == 1 && takes_strips(p.I, p.R))                                                   \
-      return launch_strips<T, true, EPI_PLAIN, false>(p, scratch, s);                                \
-    return launch_linear<T, true, false, EPI_PLAIN>(p, 1, s);                                        \
+    return dx_product<T>(p, scratch, s);                                                             \
   }                                                                                                  \
   template <> bool product_dw_huge<T>(const ProductArgs& p) {                                        \
     return sizeof(T) == 2 && takes_huge_dw(p.I, p.J) &&                                              \

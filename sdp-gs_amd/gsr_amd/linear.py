@@ -4,15 +4,20 @@
   gated_linear(x, gate_weight, up_weight, gate_bias, up_bias, activation=)
                                                 act(x Wg^T + bg) * (x Wu^T + bu)
 
-Each forward is ONE launch, with bias, activation and residual (or the product of the two halves)
-in the matrix product's epilogue.  The backward keeps nothing but the inputs: it forms the
-pre-activations again, in 32 bits, in the product that writes their gradients -- cheaper than
-storing and reading them back at a head's widths, and free of their rounding.  float32, float16
-and bfloat16 (one type per call); sums and activations in 32 bits, every result rounded once.
+Bias, activation and residual (or the product of the two halves) are in the matrix product's
+epilogue: one launch, two where weights are laid out first or a long sum is cut into ranges.  The
+backward keeps nothing but the inputs: it forms the pre-activations again, in 32 bits, in the
+product that writes their gradients -- cheaper than storing and reading them back at a head's
+widths, and free of their rounding.  float32, float16 and bfloat16 (one type per call); sums and
+activations in 32 bits, every result rounded once, 16-bit gradients before the activation rounded
+for the products that follow (their sums, the bias gradients, are not made from rounded ones).
 Results do not depend on timing.  No CPU path.
 
 A rendered feature image [C,H,W] goes in as it lies: ``fused_linear(image.reshape(C, -1).t(), W)``
 reads the channel-major memory in place.
+
+In a captured graph take gradients with ``torch.autograd.grad``, or ``backward()`` with leaves
+that no eager graph is alive for (autograd joins a leaf's stream of first use with the capture).
 """
 from __future__ import annotations
 

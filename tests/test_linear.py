@@ -55,7 +55,10 @@ SIZES = [(1, 1, 1), (1, 512, 512), (2, 3, 5), (5, 4096, 33), (17, 129, 1000), (3
          (33001, 264, 264), (16500, 72, 1032), (33001, 263, 265), (20000, 40, 200),
          # around the sizes where few rows end
          (32, 520, 640), (33, 520, 640), (63, 520, 640), (66, 520, 640), (129, 520, 640),
-         (256, 520, 640), (257, 520, 640)]
+         (256, 520, 640), (257, 520, 640),
+         # few tiles and long sums
+         (300, 4100, 130), (40, 700, 2101), (66, 1024, 2052), (4099, 600, 64), (8190, 2100, 33),
+         (20, 130, 4097)]
 
 
 @gpu
