@@ -28,7 +28,7 @@ struct ProductArgs {
   const void* bias[2];
   const void* extra;  // forward: residual; dz: dy
   int64_t extra_row;
-  void* out;  // gated dz: [I, 2J], gate then up
+  void* out;  // gated dz: [I, 2J], gate then up; dw: where there is one range, else NULL
   int64_t out_row;
   float* part;      // dw: [splits][I][J]
   // The bias gradient's partial sums, or NULL.  dw: [splits][I], row sums of A.  dz in 16 bits:

@@ -140,9 +140,14 @@ int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64
     p.r_chunk = ranges.rows;
     p.part = (float*)scratch;
     p.part_sum = db && !sums ? p.part + ranges.count * I * K : nullptr;
+    const bool direct = dw && ranges.count == 1;  // nothing to add: written as they are
+    if (direct) {
+      p.out = dw; p.out_row = K;
+    }
     if (int rc = product_dw<T>(p, ranges.count, stream)) return rc;
+    if (direct && !db) return 0;
     if (!sums) sums = p.part_sum, sum_rows = ranges.count;
-    const int64_t n = dw ? I * K : 0, n_sum = db ? I : 0;
+    const int64_t n = dw && !direct ? I * K : 0, n_sum = db ? I : 0;
     hipLaunchKernelGGL(reduce_kernel<T>, dim3((uint32_t)((n + n_sum + 63) / 64)), dim3(256), 0, stream, p.part, sums,
                        (int)ranges.count, (int)sum_rows, n, n_sum, 0, (T*)dw, (T*)db);
   } else {

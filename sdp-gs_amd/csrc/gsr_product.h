@@ -368,9 +368,15 @@ __device__ __forceinline__ uint32_t narrow_pair(float a, float b) {
   }
 }
 
+// RUN results (16 bytes of them, or 8), n of which exist.
 template <typename T, int RUN>
 __device__ __forceinline__ void store_run(T* p, const float (&v)[RUN], int64_t n) {
   if (n >= RUN) {
+    if constexpr (sizeof(T) * RUN == 8) {
+      struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t a, b; };
+      *(Bytes8*)p = Bytes8{narrow_pair<T>(v[0], v[1]), narrow_pair<T>(v[2], v[3])};
+      return;
+    }
     u32x4 w;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -680,6 +686,10 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void product_kernel(ProductArgs p,
           if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4] + bias1[k];
         }
         if constexpr (EPI == EPI_PARTIAL) {
+          if (!GATED && p.out) {  // one range: the sum is the result
+            store_run<T, RUN>((T*)p.out + i * p.out_row + j, v, n);
+            continue;
+          }
           float* part = p.part + ((int64_t)at.split * p.I + i) * (GATED ? 2 * p.J : p.J) + j;
           store_run<float, RUN>(part, v, n);
           if (GATED) store_run<float, RUN>(part + p.J, w, n);
@@ -854,14 +864,14 @@ int launch_cut(ProductArgs p, int64_t cuts, char* scratch, hipStream_t stream) {
   p.r_chunk = cut_rows(p.R, cuts);
   const int64_t splits = (p.R + p.r_chunk - 1) / p.r_chunk * p.segments;
   p.part = (float*)scratch;
-  float* sums = p.part_sum;
-  p.part_sum = nullptr;
-  const int rc = GATED ? launch_product<T, true, RCB, EPI_PARTIAL, GATED, 64, 4, 128, 1>(p, splits, stream)
-                       : launch_product<T, true, RCB, EPI_PARTIAL, GATED, 64, 4, 64, 1>(p, splits, stream);
+  ProductArgs ranges = p;
+  ranges.part_sum = nullptr;
+  ranges.out = nullptr;
+  const int rc = GATED ? launch_product<T, true, RCB, EPI_PARTIAL, GATED, 64, 4, 128, 1>(ranges, splits, stream)
+                       : launch_product<T, true, RCB, EPI_PARTIAL, GATED, 64, 4, 64, 1>(ranges, splits, stream);
   if (rc) return rc;
-  p.part_sum = sums;
   const int64_t rows = (p.I + 3) / 4;
-  if (kColumnSums<T, EPI> && sums) *p.sum_rows = rows;
+  if (kColumnSums<T, EPI> && p.part_sum) *p.sum_rows = rows;
   hipLaunchKernelGGL((finish_kernel<T, EPI, GATED>), dim3((uint32_t)((p.J + 63) / 64), (uint32_t)rows), dim3(256), 0,
                      stream, p, (uint32_t)splits);
   return hipGetLastError() == hipSuccess ? 0 : 2;

@@ -7,7 +7,7 @@ stands for are wider; `FeatureHead` maps each pixel (or each Gaussian's language
     x = x + (act(x W_g^T + b_g) * (x W_u^T + b_u)) W_d^T + b_d   `blocks` times, `hidden` wide
     y = x W_out^T + b_out                                        width -> out_features
 
-built on gsr_amd.linear: one launch for the first and the last layer and two for a block, the
+built on gsr_amd.linear: one product for the first and the last layer and two for a block, the
 image read as it lies ([3,H,W], no permuted copy).  Parameters are float32 (what FusedAdam
 updates); `dtype` is the type the products run in.  `gsr_amd.trainer.train_iteration` trains it
 with the Gaussians.

@@ -182,7 +182,10 @@ class FusedAdam(torch.optim.Adam):
     clip_grad_norm_(parameters, max_grad_norm) before it would, but inside the Adam launch: .grad
     keeps its unclipped values.  `grad_norm` is the last step's norm (a device scalar, not
     synchronised; None before the first step or without max_grad_norm).  A step in row slices
-    (begin_rows) takes the norm when it begins, so every gradient must be final by then."""
+    (begin_rows) takes the norm when it begins, so every gradient must be final by then.  All
+    gradients of a clipped step are on one device."""
+
+    max_grad_norm = grad_norm = None  # of optimizers pickled before there were these
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
                  amsgrad=False, *, maximize=False, max_grad_norm=None):
