@@ -3,10 +3,15 @@
 //
 // At these widths a tile of C has only a few steps along K, so a tiled kernel spends its time
 // filling and draining pipelines.  Here a wave loads all of its 16 NI rows at once, straight into
-// the matrix instruction's operand layout (every byte of x is read once).  The weights are first written out once as the images that LDS is to hold (16-bit parts,
-// padded with zeros to whole tiles, rows in reading order, biases among them): a tile's image goes
-// to LDS by direct loads without passing registers or needing bounds, the next one while this one
-// is worked on, and a tile's results leave as soon as they are there.
+// the matrix instruction's operand layout (every byte of x is read once).  The weights are first
+// written out once as the images that LDS is to hold (16-bit parts, padded with zeros to whole
+// tiles, rows in reading order, biases among them): a tile's image goes to LDS by direct loads
+// without passing registers or needing bounds, the next one while this one is worked on, and a
+// tile's results leave as soon as they are there.
+//
+// What bounds it: a view's layer 762048x256x512 in bfloat16 moves 1.17 GB (230 us at a copy's rate)
+// and takes 345 us forward; its products and its stores overlap only in part (156 us of the one and
+// 172 us of the other and of x's loads when timed alone).  762048x3x64 in 32 bits takes 55 us, 204 MB at 3.7 TB/s.
 #pragma once
 #include "gsr_rows.h"
 
@@ -139,130 +144,130 @@ __global__ __launch_bounds__((64 * Strip<T, KS, GATED>::kWaves), 2) void strip_k
   int buffer = 0;
 
   with_act<EPI>(p.act, [&](auto act) {
-      // One tile.  FULL: it lies within C, so its epilogue has no branch and stores kStores times.
-      auto step = [&](auto full, uint32_t tile) {
-        constexpr bool FULL = decltype(full)::value;
-        // every wave's part of this image is in LDS, and everyone has left the image before it
-        barrier();
-        const uint32_t next = tile + 1 < tile1 ? tile + 1 : tile;
-        if (images) fetch(next, buffer ^ 1);
-        if (EXTRA) load_extra(ex_next, next);
-        const int64_t j0 = (int64_t)tile * kOut;
-        const char* image = lds + buffer * S::kImage;
-        // the biases (8 of them to a row's padding) are what the sums start from
-        f32x4 acc[NI][NJ];
+    // One tile.  FULL: it lies within C, so its epilogue has no branch and stores kStores times.
+    auto step = [&](auto full, uint32_t tile) {
+      constexpr bool FULL = decltype(full)::value;
+      // every wave's part of this image is in LDS, and everyone has left the image before it
+      barrier();
+      const uint32_t next = tile + 1 < tile1 ? tile + 1 : tile;
+      if (images) fetch(next, buffer ^ 1);
+      if (EXTRA) load_extra(ex_next, next);
+      const int64_t j0 = (int64_t)tile * kOut;
+      const char* image = lds + buffer * S::kImage;
+      // the biases (8 of them to a row's padding) are what the sums start from
+      f32x4 acc[NI][NJ];
 #pragma unroll
-        for (int t = 0; t < NJ; t++) {
-          const int row = kPaired ? 32 * (t >> 1) + 8 * q + 4 * (t & 1) : 16 * t + 4 * q;
-          f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (EPI != EPI_PLAIN) bias = *(const f32x4*)(image + row / 8 * S::kRow + KS * 64 + row % 8 * 4);
+      for (int t = 0; t < NJ; t++) {
+        const int row = kPaired ? 32 * (t >> 1) + 8 * q + 4 * (t & 1) : 16 * t + 4 * q;
+        f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (EPI != EPI_PLAIN) bias = *(const f32x4*)(image + row / 8 * S::kRow + KS * 64 + row % 8 * 4);
 #pragma unroll
-          for (int u = 0; u < NI; u++) acc[u][t] = bias;
-        }
-        // the operands of kQueue reads are on their way while the products of the one before are formed
-        constexpr int kReads = KS * NJ, kQueue = kReads * kPlanes < 8 ? kReads : 8 / kPlanes;
-        s16x8 b[kQueue][kPlanes];
-        auto read = [&](int n) {
-          const int kk = n / NJ, t = n % NJ;
+        for (int u = 0; u < NI; u++) acc[u][t] = bias;
+      }
+      // the operands of kQueue reads are on their way while the products of the one before are formed
+      constexpr int kReads = KS * NJ, kQueue = kReads * kPlanes < 8 ? kReads : 8 / kPlanes;
+      s16x8 b[kQueue][kPlanes];
+      auto read = [&](int n) {
+        const int kk = n / NJ, t = n % NJ;
 #pragma unroll
-          for (int z = 0; z < kPlanes; z++)
-            b[n % kQueue][z] = *(const s16x8*)(image + z * S::kPlane + (16 * t + m) * S::kRow + (kk * 4 + q) * 16);
-        };
+        for (int z = 0; z < kPlanes; z++)
+          b[n % kQueue][z] = *(const s16x8*)(image + z * S::kPlane + (16 * t + m) * S::kRow + (kk * 4 + q) * 16);
+      };
 #pragma unroll
-        for (int n = 0; n < kQueue; n++) read(n);
-        // Two workgroups that are both at their products would stay in step and leave memory idle
-        // in between: one of the two gives way to the other.
-        if (S::kGroups == 2) {
-          if (blockIdx.x >> 8 & 1) __builtin_amdgcn_s_setprio(1);
-          else __builtin_amdgcn_s_setprio(0);
-        }
+      for (int n = 0; n < kQueue; n++) read(n);
+      // Two workgroups that are both at their products would stay in step and leave memory idle
+      // in between: one of the two gives way to the other.
+      if (S::kGroups == 2) {
+        if (blockIdx.x >> 8 & 1) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+      }
 #pragma unroll
-        for (int n = 0; n < kReads; n++) {
-          const int kk = n / NJ, t = n % NJ;
+      for (int n = 0; n < kReads; n++) {
+        const int kk = n / NJ, t = n % NJ;
 #pragma unroll
-          for (int k = 0; k < Parts<kPlanes>::kProducts; k++)
+        for (int k = 0; k < Parts<kPlanes>::kProducts; k++)
 #pragma unroll
-            for (int u = 0; u < NI; u++)
-              acc[u][t] = mfma<T>(b[n % kQueue][Parts<kPlanes>::kB[k]], a[u][kk][Parts<kPlanes>::kA[k]], acc[u][t]);
-          if (n + kQueue < kReads) read(n + kQueue);
-          __builtin_amdgcn_sched_barrier(0);  // keeps this order
-        }
-        if (S::kGroups == 2) __builtin_amdgcn_s_setprio(3);
-        if constexpr (sizeof(T) == 4) {
-          float odd = 0.0f;  // stays 0 while every result is finite
+          for (int u = 0; u < NI; u++)
+            acc[u][t] = mfma<T>(b[n % kQueue][Parts<kPlanes>::kB[k]], a[u][kk][Parts<kPlanes>::kA[k]], acc[u][t]);
+        if (n + kQueue < kReads) read(n + kQueue);
+        __builtin_amdgcn_sched_barrier(0);  // keeps this order
+      }
+      if (S::kGroups == 2) __builtin_amdgcn_s_setprio(3);
+      if constexpr (sizeof(T) == 4) {
+        float odd = 0.0f;  // stays 0 while every result is finite
+#pragma unroll
+        for (int u = 0; u < NI; u++)
+#pragma unroll
+          for (int t = 0; t < NJ; t++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) odd = fmaf(acc[u][t][v], 0.0f, odd);
+        if (odd != 0.0f) {
 #pragma unroll
           for (int u = 0; u < NI; u++)
 #pragma unroll
             for (int t = 0; t < NJ; t++)
 #pragma unroll
-              for (int v = 0; v < 4; v++) odd = fmaf(acc[u][t][v], 0.0f, odd);
-          if (odd != 0.0f) {
-#pragma unroll
-            for (int u = 0; u < NI; u++)
-#pragma unroll
-              for (int t = 0; t < NJ; t++)
-#pragma unroll
-                for (int v = 0; v < 4; v++) {
-                  const int row = t * 16 + 4 * q + v;
-                  const bool second = GATED && row >= kOut;
-                  const int64_t i = i0 + u * 16 + m, j = j0 + (second ? row - kOut : row);
-                  if (i >= p.I || j >= p.J || fabsf(acc[u][t][v]) <= 3.4e38f) continue;
-                  const float* bias = (const float*)p.bias[second ? 1 : 0];
-                  acc[u][t][v] = exact_sum((const float*)p.a, p.a_i, p.a_r, (const float*)p.b[second ? 1 : 0],
-                                           nullptr, p.b_j, p.b_r, 1, 0, i, j, 0, K) +
-                                 (EPI != EPI_PLAIN && bias ? bias[j] : 0.0f);
-                }
-          }
+              for (int v = 0; v < 4; v++) {
+                const int row = t * 16 + 4 * q + v;
+                const bool second = GATED && row >= kOut;
+                const int64_t i = i0 + u * 16 + m, j = j0 + (second ? row - kOut : row);
+                if (i >= p.I || j >= p.J || fabsf(acc[u][t][v]) <= 3.4e38f) continue;
+                const float* bias = (const float*)p.bias[second ? 1 : 0];
+                acc[u][t][v] = exact_sum((const float*)p.a, p.a_i, p.a_r, (const float*)p.b[second ? 1 : 0],
+                                         nullptr, p.b_j, p.b_r, 1, 0, i, j, 0, K) +
+                               (EPI != EPI_PLAIN && bias ? bias[j] : 0.0f);
+              }
         }
+      }
 #pragma unroll
-        for (int s = 0; s < kRuns; s++) {
-          const int64_t j = j0 + column_of(s), n = FULL ? RUN : p.J - j;
-          if (!FULL && n <= 0) continue;
-          float total[RUN] = {}, total1[RUN] = {};
+      for (int s = 0; s < kRuns; s++) {
+        const int64_t j = j0 + column_of(s), n = FULL ? RUN : p.J - j;
+        if (!FULL && n <= 0) continue;
+        float total[RUN] = {}, total1[RUN] = {};
 #pragma unroll
-          for (int u = 0; u < NI; u++) {
-            const int64_t i = i0 + u * 16 + m;
-            if (!FULL && i >= p.I) continue;
-            float v[RUN], w[RUN], e[RUN];
-            widen<T, RUN>(e, ex[u][s]);
+        for (int u = 0; u < NI; u++) {
+          const int64_t i = i0 + u * 16 + m;
+          if (!FULL && i >= p.I) continue;
+          float v[RUN], w[RUN], e[RUN];
+          widen<T, RUN>(e, ex[u][s]);
+#pragma unroll
+          for (int k = 0; k < RUN; k++) {
+            v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4];
+            if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4];
+          }
+          epilogue<T, EPI, GATED, EXTRA, decltype(act)::value, RUN>(p, i, j, n, v, w, e);
+          if (kColumnSums<T, EPI>) {
 #pragma unroll
             for (int k = 0; k < RUN; k++) {
-              v[k] = acc[u][s * (RUN / 4) + k / 4][k % 4];
-              if (GATED) w[k] = acc[u][NJ / 2 + s * (RUN / 4) + k / 4][k % 4];
-            }
-            epilogue<T, EPI, GATED, EXTRA, decltype(act)::value, RUN>(p, i, j, n, v, w, e);
-            if (kColumnSums<T, EPI>) {
-#pragma unroll
-              for (int k = 0; k < RUN; k++) {
-                total[k] += v[k];
-                if (GATED) total1[k] += w[k];
-              }
+              total[k] += v[k];
+              if (GATED) total1[k] += w[k];
             }
           }
-          if (kColumnSums<T, EPI> && p.part_sum) {
-            float* sums = p.part_sum + ((int64_t)(id / parts) * kWaves + wave) * (GATED ? 2 * p.J : p.J) + j;
-            store_sums(sums, m, n, total);
-            if (GATED) store_sums(sums + p.J, m, n, total1);
-          }
         }
-        // This wave's part of the next image has to be there.  It was asked for before the stores of
-        // this tile, the last kStores of which may go on.
-        constexpr int kStores = NI * kRuns * (EPI == EPI_DZ && GATED ? 2 : 1);
-        if (FULL) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (EXTRA) {
-#pragma unroll
-          for (int u = 0; u < NI; u++)
-#pragma unroll
-            for (int s = 0; s < kRuns; s++) ex[u][s] = ex_next[u][s];
+        if (kColumnSums<T, EPI> && p.part_sum) {
+          float* sums = p.part_sum + ((int64_t)(id / parts) * kWaves + wave) * (GATED ? 2 * p.J : p.J) + j;
+          store_sums(sums, m, n, total);
+          if (GATED) store_sums(sums + p.J, m, n, total1);
         }
-        buffer ^= 1;
-      };
-      // the tiles that lie within C, then the last ones of a ragged C
-      const uint32_t fit = i0 + 16 * NI <= p.I ? (uint32_t)(p.J / kOut) : 0;
-      uint32_t tile = tile0;
-      for (; tile < tile1 && tile < fit; tile++) step(Const<1>(), tile);
-      for (; tile < tile1; tile++) step(Const<0>(), tile);
+      }
+      // This wave's part of the next image has to be there.  It was asked for before the stores of
+      // this tile, the last kStores of which may go on.
+      constexpr int kStores = NI * kRuns * (EPI == EPI_DZ && GATED ? 2 : 1);
+      if (FULL) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (EXTRA) {
+#pragma unroll
+        for (int u = 0; u < NI; u++)
+#pragma unroll
+          for (int s = 0; s < kRuns; s++) ex[u][s] = ex_next[u][s];
+      }
+      buffer ^= 1;
+    };
+    // the tiles that lie within C, then the last ones of a ragged C
+    const uint32_t fit = i0 + 16 * NI <= p.I ? (uint32_t)(p.J / kOut) : 0;
+    uint32_t tile = tile0;
+    for (; tile < tile1 && tile < fit; tile++) step(Const<1>(), tile);
+    for (; tile < tile1; tile++) step(Const<0>(), tile);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing arrives in LDS that is another's
   });
 }
