@@ -279,12 +279,33 @@ def test_same_bits_every_time_and_on_another_stream(pair):
 
 
 @gpu
+def test_two_calls_at_once():
+    """Calls on two streams, of sizes that need scratch memory, do not disturb each other."""
+    sizes = [(300, 2100, 130), (33000, 64, 200)]
+    ds = [ref.inputs(20 + i, *sizes[i], torch.bfloat16, "cuda") for i in range(2)]
+    want = [_run(dict(d), "silu") for d in ds]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_run(dict(ds[i]), "silu"))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for n in g:
+                assert torch.equal(g[n], want[i][n]), (i, n)
+
+
+@gpu
 @pytest.mark.parametrize("pair", [False, True])
-def test_captured_and_replayed(pair):
+@pytest.mark.parametrize("t,M,K", [(torch.float32, 700, 40), (torch.bfloat16, 3000, 2100),
+                                   (torch.float16, 33000, 40)])
+def test_captured_and_replayed(pair, t, M, K):
     """Forward and backward in a graph, replayed on new values with eager calls between: each
     replay has the eager call's bits.  Two graphs of the same shapes live side by side."""
-    t = torch.float32
-    d = ref.inputs(12, 700, 40, 72, t, "cuda", gated_pair=pair)
+    d = ref.inputs(12, M, K, 72, t, "cuda", gated_pair=pair)
     _run(dict(d), "silu")  # builds, allocates
     torch.cuda.synchronize()
     names = [n for n in ("x", "w0", "w1", "b0", "b1") if n in d]
@@ -299,7 +320,7 @@ def test_captured_and_replayed(pair):
         graphs.append((g, s, out))
     for k in range(4):
         for i, (g, s, out) in enumerate(graphs):
-            new = ref.inputs(100 + 2 * k + i, 700, 40, 72, t, "cuda", gated_pair=pair)
+            new = ref.inputs(100 + 2 * k + i, M, K, 72, t, "cuda", gated_pair=pair)
             for n in s:
                 s[n].copy_(new[n])
             g.replay()
