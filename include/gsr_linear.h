@@ -10,7 +10,7 @@
  *   x:  x_row = distance between rows, x_col = distance between columns; one of them is 1
  *       (x_col = 1: rows as they come; x_row = 1: a channel-major image [K,H,W] read in place)
  *   w, residual, y, dy, gradients: rows contiguous, any row stride >= the row's length
- * M = 0 is a no-op (weight gradients are set to zero); K and N are at least 1.
+ * M = 0 is a no-op (weight gradients are set to zero); K is 1 to 2^22, N 1 to 2^21, M up to 2^36.
  * Every launch goes to `stream` on the current device.  scratch: device memory of the size the
  * matching *_scratch_bytes function gives (NULL for 0), 256-byte aligned, untouched by others until
  * the call's work is done; it holds nothing between calls.  Results do not depend on timing (no atomics).

@@ -8,6 +8,10 @@
 // digits than the result has (64-bit adds are far from the bound: two per 4 bytes read).  Whoever
 // needs the norm adds the at most kGrid partial sums of each launch in their order: no atomics, so
 // the same gradients give the same bits.
+//
+// HBM bounds both: of 62M floats (248 MB) the norm takes 41 us (6.0 TB/s), a call that scales 114
+// (read, then read and write: 744 MB, 6.5 TB/s, some of them from the last-level cache), one that
+// finds nothing to scale 42.  60 small tensors: the host's call.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
