@@ -114,6 +114,14 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _weight_pair(gate, up, K):
+    """Both weights as rows of one distance."""
+    wg, wu = _rows(gate, K), _rows(up, K)
+    if _row_stride(wg) != _row_stride(wu):
+        wg, wu = wg.contiguous(), wu.contiguous()
+    return wg, wu
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
@@ -134,16 +142,19 @@ class _Linear(torch.autograd.Function):
                     y.data_ptr(), N, _ptr(scratch), _lib.raw_stream(x.device)), "gsr_linear")
         if ctx is not None:
             ctx.save_for_backward(xm, w, b)
-            ctx.args = (x.shape, x_row, x_col, act)
+            ctx.args = (x.shape, act)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        # what comes back may lie otherwise than what was saved (saved_tensors_hooks, save_on_cpu)
         xm, w, b = ctx.saved_tensors
-        shape, x_row, x_col, act = ctx.args
+        shape, act = ctx.args
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         (N, K), M = w.shape, xm.shape[0]
+        xm, x_row, x_col = _x_matrix(xm, K)
+        w, b = _rows(w, K), None if b is None else b.contiguous()
         kind, dev = xm.dtype, xm.device
         dx = torch.empty(shape, dtype=kind, device=dev) if need_x else None
         dw = torch.empty((N, K), dtype=kind, device=dev) if need_w else None
@@ -167,9 +178,7 @@ class _Gated(torch.autograd.Function):
         N, K = gate.shape
         xm = _rows(x, K)
         M = xm.shape[0]
-        wg, wu = _rows(gate, K), _rows(up, K)
-        if _row_stride(wg) != _row_stride(wu):
-            wg, wu = wg.contiguous(), wu.contiguous()
+        wg, wu = _weight_pair(gate, up, K)
         bg = None if gate_bias is None else gate_bias.contiguous()
         bu = None if up_bias is None else up_bias.contiguous()
         h = x.new_empty(x.shape[:-1] + (N,))
@@ -193,6 +202,8 @@ class _Gated(torch.autograd.Function):
         shape, act = ctx.args
         need = ctx.needs_input_grad
         (N, K), M = wg.shape, xm.shape[0]
+        xm, (wg, wu) = _rows(xm, K), _weight_pair(wg, wu, K)  # they may lie otherwise than when saved
+        bg, bu = (None if b is None else b.contiguous() for b in (bg, bu))
         kind, dev = xm.dtype, xm.device
         need_w, need_b = need[1] or need[2], need[3] or need[4]
         dx = torch.empty(shape, dtype=kind, device=dev) if need[0] else None
