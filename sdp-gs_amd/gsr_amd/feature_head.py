@@ -10,7 +10,11 @@ stands for are wider; `FeatureHead` maps each pixel (or each Gaussian's language
 built on gsr_amd.linear: one product for the first and the last layer and two for a block, the
 image read as it lies ([3,H,W], no permuted copy).  Parameters are float32 (what FusedAdam
 updates); `dtype` is the type the products run in.  `gsr_amd.trainer.train_iteration` trains it
-with the Gaussians.
+with the Gaussians, in float32 or bfloat16.  A float16 head is for use only: a mean over a view's
+pixels gives each output a gradient near 1 / (pixels x features), 2e-9 for 762048 x 512, below
+float16's smallest step of 6e-8.  No factor on the loss helps in general: one that lifts these
+gradients into the type's range can lift their sums over the pixels, the weights' gradients, out
+of it.
 """
 from __future__ import annotations
 
@@ -66,9 +70,16 @@ class FeatureHead(torch.nn.Module):
             return self.rows(flat[:, pixels].t())
         return self.rows(flat.t()).reshape(image.shape[1], image.shape[2], self.out_features)
 
+    def refuse_training(self):
+        """Raise ValueError if this head's type cannot hold a view's gradients."""
+        if self.dtype is torch.float16:
+            raise ValueError("FeatureHead: a float16 head is not trained here, the gradients of a "
+                             "mean over pixels vanish in that type; use bfloat16 or float32")
+
     def training_setup(self, lr=1e-3):
         """The head's own FusedAdam (its parameters are not Gaussians: densification must not see
         them in the model's groups)."""
         from .optim import FusedAdam
+        self.refuse_training()
         self.optimizer = FusedAdam(self.parameters(), lr=lr, eps=1e-15)
         return self.optimizer

@@ -134,12 +134,15 @@ def feature_loss(decoded, target):
 def train_iteration(model, cam, gt_image, depth_mono, bg, args: OptArgs, iteration: int,
                     extent: float, pipe=None, feature_head=None, gt_feature=None):
     """One reference iteration on one camera.  Returns the loss tensor (not synchronised).
-    feature_head (gsr_amd.feature_head.FeatureHead with its training_setup done) and gt_feature,
-    the wide features it should give: [H,W,D], or ([S,D], pixels [S]) for some pixels only.  The
-    loss gains args.feature_weight times feature_loss, and the head takes its own Adam step."""
+    feature_head (gsr_amd.feature_head.FeatureHead in float32 or bfloat16, its training_setup done)
+    and gt_feature, the wide features it should give: [H,W,D], or ([S,D], pixels [S]) for some
+    pixels only.  The loss gains args.feature_weight times feature_loss, and the head takes its own
+    Adam step."""
     from gaussian_renderer import render
     if (feature_head is None) != (gt_feature is None):
         raise ValueError("train_iteration: feature_head and gt_feature belong together")
+    if feature_head is not None:
+        feature_head.refuse_training()
     pipe = pipe or _Pipe()
     pkg = render(cam, model, pipe, bg, args)
     loss = _view_loss(pkg, gt_image, depth_mono, args)
