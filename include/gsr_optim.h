@@ -62,7 +62,8 @@ int gsr_adam_step_scaled(int n_tensors, float* const* params, const float* const
 /* The norm of all elements of n_tensors >= 1 gradients together (torch.nn.utils.clip_grad_norm_'s
  * total norm).  grads[t]: device pointer to numel[t] (0 allowed) contiguous elements of dtype[t]
  * (GSR_F32 / GSR_F16 / GSR_BF16, gsr_linear.h); sums are held in 64 bits.  norm: device float;
- * scale (or NULL): device float receiving min(1, max_norm / (norm + 1e-6)), NaN if the norm is.
+ * scale (or NULL): device float receiving min(1, max_norm / (norm + 1e-6)), NaN if the norm is;
+ * max_norm >= 0 then.
  * Any number of tensors: GSR_CLIP_LAUNCH_TENSORS to a launch.  scratch: device memory of
  * gsr_grad_norm_scratch_bytes(n_tensors) bytes, 8-byte aligned, holding nothing between calls.
  * The same gradients give the same bits.  0 ok, 1 invalid arguments, 2 launch error. */

@@ -247,6 +247,7 @@ extern "C" int gsr_grad_norm(int n_tensors, const void* const* grads, const int6
                              const int* dtype, int norm_type, float max_norm, float* norm,
                              float* scale, void* scratch, void* stream) {
   if (n_tensors < 1 || !grads || !numel || !dtype || !norm || !scratch) return 1;
+  if (scale && !(max_norm >= 0.0f)) return 1;  // a negative factor would turn the gradients round
   void* const* g = const_cast<void* const*>(grads);
   hipStream_t s = (hipStream_t)stream;
   double* part = (double*)scratch;

@@ -64,6 +64,13 @@ def _norm_code(norm_type):
     return _NORMS[float(norm_type)]
 
 
+def _limit(max_norm, name):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:  # NaN is refused too
+        raise ValueError(f"{name} must be at least 0, not {max_norm}")
+    return max_norm
+
+
 class _CTensors:
     """The tensors that hold elements, checked, as the C entries take them; one with gaps between
     its elements as a copy.  (Each attribute of each tensor is asked for once: a head has many.)"""
@@ -154,9 +161,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     a norm that is NaN makes every gradient NaN, unless error_if_nonfinite (which waits for the
     norm) raises first.  Gradients must not share memory with each other."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must be at least 0, not {max_norm}")
+    max_norm = _limit(max_norm, "max_norm")
     code = _norm_code(norm_type)
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     c = _CTensors(grads)
@@ -191,8 +196,8 @@ class FusedAdam(torch.optim.Adam):
                  amsgrad=False, *, maximize=False, max_grad_norm=None):
         if amsgrad or maximize:
             raise ValueError("FusedAdam implements Adam without amsgrad / maximize")
-        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
-            raise ValueError(f"max_grad_norm must be at least 0, not {max_grad_norm}")
+        if max_grad_norm is not None:
+            _limit(max_grad_norm, "max_grad_norm")
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                          amsgrad=False, foreach=False)
         self._mailbox = {}     # device -> pinned int32 [1]: 1 = the step's launches skipped it
@@ -249,6 +254,7 @@ class FusedAdam(torch.optim.Adam):
         self._resolve_pending()
         grads = None
         if self.max_grad_norm is not None:  # refused before any step count advances
+            limit = _limit(self.max_grad_norm, "max_grad_norm")  # it may have been set since __init__
             grads = _CTensors([p.grad for group in self.param_groups for p in group["params"]
                                if p.grad is not None])
         batches = {}
@@ -307,7 +313,7 @@ class FusedAdam(torch.optim.Adam):
         scale = None
         if grads is not None and grads.n:
             scale = torch.empty(1, dtype=torch.float32, device=grads.device)
-            self.grad_norm = _norm_and_scale(grads, _NORMS[2.0], self.max_grad_norm, scale)
+            self.grad_norm = _norm_and_scale(grads, _NORMS[2.0], limit, scale)
         return {"batches": batches, "skips": skips, "states": states, "issued": False,
                 "scale": scale}
 
