@@ -98,31 +98,35 @@ def _optimizer_step(model, reducer=None, args=None, head=None):
     """optimizer.step(); with a multi-GPU reducer FusedAdam takes the ranks' summed fault
     snapshot as its skip decision (any rank failed -> every rank skips).
     args.max_grad_norm: the gradients clipped by their global norm -- inside the Adam launch, or,
-    where a head's are part of the norm (or the optimizer is another), in place before it."""
+    where a head's are part of the norm (or the optimizer is another), in place before it; for this
+    step it takes the place of the optimizers' own limits."""
     from . import _lib
     from .optim import FusedAdam, clip_grad_norm_
     opt = model.optimizer
     limit = None if args is None else getattr(args, "max_grad_norm", None)
     skip = reducer.skip_flag() if reducer is not None else None
-    if limit is not None and (head is not None or not isinstance(opt, FusedAdam)):
-        clip_grad_norm_([p for g in opt.param_groups for p in g["params"]]
-                        + ([] if head is None else list(head.parameters())), limit)
-        limit = None
-    if head is not None:
-        if skip is None:  # one snapshot for both optimizers: both step or neither does
-            skip = torch.empty(1, dtype=torch.float32, device=model.get_xyz.device)
-            _lib.step_guard(skip)
-        head.optimizer.step(skip=skip)
-    if isinstance(opt, FusedAdam):
-        own = opt.max_grad_norm
-        if limit is not None:
-            opt.max_grad_norm = limit
-        try:
+    fused = [o for o in (opt, getattr(head, "optimizer", None)) if isinstance(o, FusedAdam)]
+    own = [o.max_grad_norm for o in fused]
+    if limit is not None:
+        inside = head is None and isinstance(opt, FusedAdam)
+        if not inside:
+            clip_grad_norm_([p for g in opt.param_groups for p in g["params"]]
+                            + ([] if head is None else list(head.parameters())), limit)
+        for o in fused:
+            o.max_grad_norm = limit if inside else None
+    try:
+        if head is not None:
+            if skip is None:  # one snapshot for both optimizers: both step or neither does
+                skip = torch.empty(1, dtype=torch.float32, device=model.get_xyz.device)
+                _lib.step_guard(skip)
+            head.optimizer.step(skip=skip)
+        if isinstance(opt, FusedAdam):
             opt.step(skip=skip)
-        finally:
-            opt.max_grad_norm = own
-    else:
-        opt.step()
+        else:
+            opt.step()
+    finally:
+        for o, m in zip(fused, own):
+            o.max_grad_norm = m
 
 
 def feature_loss(decoded, target):

@@ -39,3 +39,59 @@ def test_a_float16_head_is_not_trained():
                                 feature_head=head, gt_feature=torch.zeros(5, 6, 8))
     for t in (torch.float32, torch.bfloat16):
         FeatureHead(8, width=4, blocks=1, dtype=t, device="cpu").training_setup()
+
+
+class _Head(torch.nn.Linear):
+    def __init__(self, device, limit):
+        super().__init__(3, 2, device=device)
+        from gsr_amd.optim import FusedAdam
+        self.optimizer = FusedAdam(self.parameters(), lr=1e-2, max_grad_norm=limit)
+
+
+def _pair(device, limit, with_head):
+    """A model and a head of a few parameters whose optimizers have a limit of their own."""
+    from types import SimpleNamespace
+
+    from gsr_amd.optim import FusedAdam
+    g = torch.Generator().manual_seed(5)
+    p = torch.nn.Parameter(torch.randn(7, 3, generator=g).to(device))
+    model = SimpleNamespace(optimizer=FusedAdam([p], lr=1e-2, max_grad_norm=limit), get_xyz=p)
+    head = _Head(device, limit) if with_head else None
+    ps = [p] + (list(head.parameters()) if with_head else [])
+    with torch.no_grad():
+        for q in ps:
+            q.copy_(torch.randn(q.shape, generator=g))
+            q.grad = torch.randn(q.shape, generator=g).to(device)
+    return model, head, ps
+
+
+@pytest.mark.parametrize("with_head", [False, True])
+@pytest.mark.parametrize("limit", [None, 0.5])
+def test_the_arguments_limit_takes_the_place_of_the_optimizers_own(monkeypatch, with_head, limit):
+    """What each optimizer's step clips by, and afterwards its own limit as before."""
+    from gsr_amd import _lib, optim
+    model, head, ps = _pair("cpu", 0.25, with_head)
+    steps, clips = [], []
+    monkeypatch.setattr(optim.FusedAdam, "step", lambda self, skip=None: steps.append((self, self.max_grad_norm)))
+    monkeypatch.setattr(optim, "clip_grad_norm_", lambda params, m: clips.append((len(params), m)))
+    monkeypatch.setattr(_lib, "step_guard", lambda slot: None)
+    trainer._optimizer_step(model, args=trainer.OptArgs(max_grad_norm=limit), head=head)
+    inside = 0.25 if limit is None else None if with_head else limit
+    assert steps == ([(head.optimizer, inside)] if with_head else []) + [(model.optimizer, inside)]
+    assert clips == ([(len(ps), limit)] if with_head and limit is not None else [])
+    assert model.optimizer.max_grad_norm == 0.25
+    assert head is None or head.optimizer.max_grad_norm == 0.25
+
+
+@gpu
+@pytest.mark.parametrize("with_head", [False, True])
+def test_a_step_is_clipped_once(with_head):
+    """With an own limit far below the arguments' the step has the bits of one without."""
+    results = []
+    for limit in (None, 1e-4):
+        model, head, ps = _pair("cuda", limit, with_head)
+        trainer._optimizer_step(model, args=trainer.OptArgs(max_grad_norm=0.5), head=head)
+        opts = [model.optimizer] + ([head.optimizer] if with_head else [])
+        results.append([p.detach().clone() for p in ps]
+                       + [v["exp_avg"] for o in opts for v in o.state.values()])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
