@@ -186,7 +186,7 @@ class FusedAdam(torch.optim.Adam):
     """max_grad_norm: clip by the global 2-norm of every parameter's gradient in each step, as
     clip_grad_norm_(parameters, max_grad_norm) before it would, but inside the Adam launch: .grad
     keeps its unclipped values.  `grad_norm` is the last step's norm (a device scalar, not
-    synchronised; None before the first step or without max_grad_norm).  A step in row slices
+    synchronised; None before the first step and after one without clipping).  A step in row slices
     (begin_rows) takes the norm when it begins, so every gradient must be final by then.  All
     gradients of a clipped step are on one device."""
 
@@ -310,8 +310,10 @@ class FusedAdam(torch.optim.Adam):
             else:
                 skips[dev] = (skip.data_ptr(), box)
         states = [self.state[it[0]] for its in batches.values() for it in its]
-        scale = None
-        if grads is not None and grads.n:
+        scale = self.grad_norm = None  # a step that is not clipped has no norm
+        if grads is not None and not grads.n:
+            self.grad_norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
+        elif grads is not None:
             scale = torch.empty(1, dtype=torch.float32, device=grads.device)
             self.grad_norm = _norm_and_scale(grads, _NORMS[2.0], limit, scale)
         return {"batches": batches, "skips": skips, "states": states, "issued": False,

@@ -110,8 +110,8 @@ def _optimizer_step(model, reducer=None, args=None, head=None):
     if limit is not None:
         inside = head is None and isinstance(opt, FusedAdam)
         if not inside:
-            clip_grad_norm_([p for g in opt.param_groups for p in g["params"]]
-                            + ([] if head is None else list(head.parameters())), limit)
+            norm = clip_grad_norm_([p for g in opt.param_groups for p in g["params"]]
+                                   + ([] if head is None else list(head.parameters())), limit)
         for o in fused:
             o.max_grad_norm = limit if inside else None
     try:
@@ -124,6 +124,9 @@ def _optimizer_step(model, reducer=None, args=None, head=None):
             opt.step(skip=skip)
         else:
             opt.step()
+        if limit is not None and not inside:
+            for o in fused:
+                o.grad_norm = norm
     finally:
         for o, m in zip(fused, own):
             o.max_grad_norm = m

@@ -95,3 +95,31 @@ def test_a_step_is_clipped_once(with_head):
         results.append([p.detach().clone() for p in ps]
                        + [v["exp_avg"] for o in opts for v in o.state.values()])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_a_norm_is_of_the_last_step():
+    """A step without clipping leaves no norm behind, one without gradients that of nothing."""
+    from gsr_amd.optim import FusedAdam
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = FusedAdam([p], max_grad_norm=1.0)
+    for limit, want in ((1.0, 0.0), (None, None)):
+        opt.grad_norm = torch.tensor(7.0)
+        opt.max_grad_norm = limit
+        opt.step()
+        assert opt.grad_norm is None if want is None else float(opt.grad_norm) == want
+
+
+@gpu
+def test_the_norm_of_a_step_with_a_head_is_that_of_both():
+    from gsr_amd.optim import grad_norm
+    model, head, ps = _pair("cuda", 1.0, True)
+    want = grad_norm([q.grad for q in ps])
+    trainer._optimizer_step(model, args=trainer.OptArgs(max_grad_norm=0.5), head=head)
+    assert torch.equal(model.optimizer.grad_norm, want) and torch.equal(head.optimizer.grad_norm, want)
+    for q in ps:
+        q.grad = torch.zeros_like(q)
+    trainer._optimizer_step(model, args=trainer.OptArgs(), head=head)  # each by its own limit
+    assert float(model.optimizer.grad_norm) == float(head.optimizer.grad_norm) == 0.0
+    model.optimizer.max_grad_norm = None
+    trainer._optimizer_step(model, args=trainer.OptArgs())
+    assert model.optimizer.grad_norm is None
