@@ -11,7 +11,8 @@ product that writes their gradients -- cheaper than storing and reading them bac
 widths, and free of their rounding.  float32, float16 and bfloat16 (one type per call); sums and
 activations in 32 bits, every result rounded once, 16-bit gradients before the activation rounded
 for the products that follow (their sums, the bias gradients, are not made from rounded ones).
-Results do not depend on timing.  No CPU path.
+Results do not depend on timing.  Reverse mode only: a tangent (torch.autograd.forward_ad) is
+refused.  No CPU path.
 
 A rendered feature image [C,H,W] goes in as it lies: ``fused_linear(image.reshape(C, -1).t(), W)``
 reads the channel-major memory in place.
@@ -22,6 +23,7 @@ that no eager graph is alive for (autograd joins a leaf's stream of first use wi
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -108,6 +110,13 @@ def _ptr(t):
 
 def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _refuse_tangents(*tensors):
+    """A dual tensor needs no gradient, so nothing else would notice that its tangent is lost."""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+           for t in tensors):
+        raise NotImplementedError("gsr fused products have no forward-mode derivative")
 
 
 def _wants_grad(*tensors):
@@ -227,6 +236,8 @@ class _Gated(torch.autograd.Function):
 def fused_linear(x, weight, bias=None, *, activation="none", residual=None):
     """activation(x @ weight.T + bias) + residual.  x [..., K], weight [N, K], bias [N], residual
     [..., N] (the result's shape); differentiable once in each of them."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight, bias, residual)
     if not (_base_fits(x, weight, activation) and _fits(bias, weight.shape[:1], x)
             and _fits(residual, x.shape[:-1] + weight.shape[:1], x)):
         _refuse(x, weight, "weight", lambda N, K: [
@@ -239,6 +250,8 @@ def fused_linear(x, weight, bias=None, *, activation="none", residual=None):
 def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, activation="silu"):
     """activation(x @ gate_weight.T + gate_bias) * (x @ up_weight.T + up_bias), both products in
     one pass over x.  x [..., K], weights [N, K], biases [N]; differentiable once in each."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, gate_weight, up_weight, gate_bias, up_bias)
     if not (_base_fits(x, gate_weight, activation) and up_weight is not None
             and _fits(up_weight, gate_weight.shape, x) and _fits(gate_bias, gate_weight.shape[:1], x)
             and _fits(up_bias, gate_weight.shape[:1], x)):
