@@ -39,7 +39,9 @@ int gsr_linear(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_
 /* Gradients of gsr_linear: with z = x w^T + bias (computed again, so a forward keeps nothing)
  * and dz = dy act'(z): dx = dz w [M,K], dw = dz^T x [N,K], dbias = the column sums of dz [N], all
  * contiguous; any of them may be NULL.  The residual's gradient is dy.  16-bit dz is rounded for the
- * products, not for its sums.  need_dw: whether dw or dbias is going to be asked for. */
+ * products, not for its sums.  need_dw: GSR_NEED_DW if dw is going to be asked for (with dbias or
+ * not), GSR_NEED_DB if dbias alone, 0 if neither. */
+enum { GSR_NEED_DW = 1, GSR_NEED_DB = 2 };
 size_t gsr_linear_backward_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N, int act,
                                          int need_dw);
 int gsr_linear_backward(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,
@@ -56,7 +58,7 @@ int gsr_gated(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t
 
 /* Gradients of gsr_gated (g, u computed again): dg = dh u act'(g), du = dh act(g);
  * dx = dg wg + du wu [M,K]; dw [2N,K] = the gradients of wg and then wu; db [2N] likewise.  Any of
- * them may be NULL. */
+ * them may be NULL.  need_dw as above. */
 size_t gsr_gated_backward_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N, int need_dw);
 int gsr_gated_backward(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_t x_row,
                        const void* wg, const void* wu, int64_t w_row, const void* bg,

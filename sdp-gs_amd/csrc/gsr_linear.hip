@@ -120,6 +120,10 @@ int activation_gradients(ProductArgs p, bool gated, bool need_db, char*& scratch
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
+// A bias gradient that is summed beside the weight gradients comes, where these are not asked for,
+// with those of a few of x's columns: the same ranges, the same bits, without the product's work.
+int64_t columns_of(int64_t K, bool dw) { return dw || K < 8 ? K : 8; }
+
 // The weight gradients: partial products over ranges of x's rows, then their sum.  The bias gradient
 // is dz's sum beside them, or that of `sum_rows` rows of `sums`.
 template <typename T>
@@ -137,10 +141,11 @@ int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64
     p.b[0] = x; p.b_j = x_col; p.b_r = x_row;
     p.I = I; p.J = K; p.R = M; p.segments = 1;
     const Ranges ranges = ranges_of(I, K, M, product_dw_huge<T>(p));
+    p.J = columns_of(K, dw);
     p.r_chunk = ranges.rows;
     p.part = (float*)scratch;
-    p.part_sum = db && !sums ? p.part + ranges.count * I * K : nullptr;
     const bool direct = dw && ranges.count == 1;  // nothing to add: written as they are
+    p.part_sum = !db || sums ? nullptr : direct ? p.part : p.part + ranges.count * I * p.J;
     if (direct) {
       p.out = dw; p.out_row = K;
     }
@@ -157,17 +162,21 @@ int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-size_t partial_bytes(int64_t M, int64_t K, int64_t I) {
+// What weight_gradients takes; dw: they are asked for, not the bias gradient alone.
+size_t partial_bytes(int64_t M, int64_t K, int64_t I, bool dw) {
   if (M == 0) return 0;
-  int64_t n = ranges_of(I, K, M, false).count;
-  if (takes_huge_dw(I, K) && ranges_of(I, K, M, true).count > n) n = ranges_of(I, K, M, true).count;
-  return (size_t)n * I * (K + 1) * 4;
+  auto of = [&](bool huge) {
+    const int64_t n = ranges_of(I, K, M, huge).count;
+    return n * (columns_of(K, dw && n > 1) + 1);  // one range is written where it belongs
+  };
+  const int64_t small = of(false), huge = takes_huge_dw(I, K) ? of(true) : 0;
+  return (size_t)(small > huge ? small : huge) * I * 4;
 }
 
 // Scratch of a backward, in order: the gradients before the activation, their sums, then what one
 // product at a time needs (the weights' images, the partial sums).
 template <typename T>
-size_t backward_bytes(int64_t M, int64_t K, int64_t N, bool gated, bool has_dz, bool need_dw) {
+size_t backward_bytes(int64_t M, int64_t K, int64_t N, bool gated, bool has_dz, int need_dw) {
   const int64_t width = gated ? 2 * N : N;
   const bool column_sums = has_dz && need_dw && sizeof(T) == 2;
   const ColumnSums c(M, width);
@@ -175,7 +184,7 @@ size_t backward_bytes(int64_t M, int64_t K, int64_t N, bool gated, bool has_dz, 
   if (column_sums) most += c.bytes();
   const size_t dx = dx_scratch<T>(M, K, N, gated ? 2 : 1);
   most = dx > most ? dx : most;
-  const size_t dw = need_dw ? partial_bytes(M, K, width) : 0;
+  const size_t dw = need_dw ? partial_bytes(M, K, width, need_dw != GSR_NEED_DB) : 0;
   most = dw > most ? dw : most;
   return (has_dz ? (size_t)up(M * width * sizeof(T), 256) : 0) + (column_sums ? c.kept_bytes() : 0) + most;
 }

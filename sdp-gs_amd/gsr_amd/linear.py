@@ -108,6 +108,10 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _need(weight, bias):
+    return 1 if weight else 2 if bias else 0  # GSR_NEED_DW / GSR_NEED_DB
+
+
 def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -172,7 +176,7 @@ class _Linear(torch.autograd.Function):
             g = _rows(dy, N)
             L = _lib.load()
             scratch = _scratch(L.gsr_linear_backward_scratch_bytes(
-                DTYPES[kind], M, K, N, act, int(need_w or need_b)), dev)
+                DTYPES[kind], M, K, N, act, _need(need_w, need_b)), dev)
             with _lib.on_device(dev):
                 _check(L.gsr_linear_backward(
                     DTYPES[kind], M, K, N, xm.data_ptr(), x_row, x_col, w.data_ptr(),
@@ -222,7 +226,7 @@ class _Gated(torch.autograd.Function):
             g = _rows(dh, N)
             L = _lib.load()
             scratch = _scratch(L.gsr_gated_backward_scratch_bytes(
-                DTYPES[kind], M, K, N, int(need_w or need_b)), dev)
+                DTYPES[kind], M, K, N, _need(need_w, need_b)), dev)
             with _lib.on_device(dev):
                 _check(L.gsr_gated_backward(
                     DTYPES[kind], M, K, N, xm.data_ptr(), _row_stride(xm), wg.data_ptr(),
