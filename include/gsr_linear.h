@@ -6,7 +6,8 @@
  *
  * Shapes: x [M,K], w [N,K] (row n holds output n's weights), bias [N], residual / y / dy [M,N].
  * dtype is one of GSR_F32 / GSR_F16 / GSR_BF16 for every operand of a call; sums and activations
- * are held in 32 bits and each output is rounded once.  Strides are in elements.
+ * are held in 32 bits and each output is rounded once.  GSR_F32 operands below 2^-110 are held to
+ * 2^-134, larger ones exactly.  Strides are in elements.
  *   x:  x_row = distance between rows, x_col = distance between columns; one of them is 1
  *       (x_col = 1: rows as they come; x_row = 1: a channel-major image [K,H,W] read in place)
  *   w, residual, y, dy, gradients: rows contiguous, any row stride >= the row's length
@@ -38,8 +39,9 @@ int gsr_linear(int dtype, int64_t M, int64_t K, int64_t N, const void* x, int64_
 
 /* Gradients of gsr_linear: with z = x w^T + bias (computed again, so a forward keeps nothing)
  * and dz = dy act'(z): dx = dz w [M,K], dw = dz^T x [N,K], dbias = the column sums of dz [N], all
- * contiguous; any of them may be NULL.  The residual's gradient is dy.  16-bit dz is rounded for the
- * products, not for its sums.  need_dw: GSR_NEED_DW if dw is going to be asked for (with dbias or
+ * contiguous; any of them may be NULL.  The residual's gradient is dy.  16-bit dz of an activation is
+ * rounded for the products, not for its sums: in GSR_F16 it is infinite beyond 65504 and 0 up to 2^-25
+ * there, and dx and dw are what such factors give.  need_dw: GSR_NEED_DW if dw is going to be asked for (with dbias or
  * not), GSR_NEED_DB if dbias alone, 0 if neither. */
 enum { GSR_NEED_DW = 1, GSR_NEED_DB = 2 };
 size_t gsr_linear_backward_scratch_bytes(int dtype, int64_t M, int64_t K, int64_t N, int act,

@@ -7,7 +7,8 @@
 // consecutive j of one i and leave as 16-byte stores.
 //
 // 32-bit operands: a float is the exact sum of three bfloat16 parts (8 + 8 + 8 bits, each the
-// rounded remainder of the one before).  Six of the nine products of parts are formed, those of
+// rounded remainder of the one before) from 2^-110 on; below that the last parts pass the type's
+// smallest step, 2^-133, and the float is held to half of it.  Six of the nine products of parts are formed, those of
 // 2^-16 or more; the three left out are below 2^-24 of the product together, a float product's own
 // rounding.  At 6/16 the rate of the 16-bit instruction that is 2.6x the float instruction's rate.
 // Parts of an infinity or a NaN do not sum to it, so a result that is not finite is computed again
