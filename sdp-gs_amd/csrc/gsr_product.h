@@ -785,7 +785,7 @@ int launch_gated(const ProductArgs& p, hipStream_t stream) {
 template <typename T>
 int64_t cuts_of(int64_t I, int64_t J, int64_t R, int64_t segments) {
   const int64_t tiles = (I + 63) / 64 * ((J + 63) / 64) * segments;
-  if (tiles > 128 || R < (sizeof(T) == 4 ? 512 : 2048)) return 1;
+  if (tiles < 1 || tiles > 128 || R < (sizeof(T) == 4 ? 512 : 2048)) return 1;  // no rows: no tiles
   const int64_t most = R / 256, want = 512 / tiles;
   return want < most ? want : most;
 }
