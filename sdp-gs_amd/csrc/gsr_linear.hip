@@ -50,8 +50,13 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* part, const fl
 
 template <typename T>
 __global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e < n) p[e] = from_f<T>(0.0f);
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256)
+    p[e] = from_f<T>(0.0f);
+}
+template <typename T>
+void zero(void* p, int64_t n, hipStream_t stream) {
+  const int64_t groups = (n + 255) / 256;
+  hipLaunchKernelGGL(zero_kernel<T>, dim3((uint32_t)(groups < 65536 ? groups : 65536)), dim3(256), 0, stream, (T*)p, n);
 }
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
@@ -135,8 +140,8 @@ int weight_gradients(const void* dz, int64_t dz_row, int64_t M, int64_t K, int64
                      int64_t x_row, int64_t x_col, void* dw, void* db, const float* sums, int64_t sum_rows,
                      char* scratch, hipStream_t stream) {
   if (M == 0) {
-    if (dw) hipLaunchKernelGGL(zero_kernel<T>, dim3((I * K + 255) / 256), dim3(256), 0, stream, (T*)dw, I * K);
-    if (db) hipLaunchKernelGGL(zero_kernel<T>, dim3((I + 255) / 256), dim3(256), 0, stream, (T*)db, I);
+    if (dw) zero<T>(dw, I * K, stream);
+    if (db) zero<T>(db, I, stream);
     return hipGetLastError() == hipSuccess ? 0 : 2;
   }
   ProductArgs p{};

@@ -726,12 +726,43 @@ bool takes_direct(const ProductArgs& p) {
   return sizeof(T) == 2 && bits % 16 == 0;
 }
 
+// A launch of 2^32 threads or more is refused, or begins only as many as are left over that without
+// an error.
+constexpr int64_t kMostThreads = 0xffffffff;
+// So more rows than this are taken in slabs, of 256 threads for 64 rows or more.
+constexpr int64_t kSlabRows = 1 << 29;
+
+// f(the product of some of its rows) over slabs of about the same size (of more rows than those that
+// choose a kernel or ask for scratch); `width` of the partial column sums, if it makes any.
+template <typename T, typename F>
+int in_slabs(const ProductArgs& p, int64_t width, F f) {
+  if (p.I <= kSlabRows) return f(p);
+  const int64_t slabs = (p.I + kSlabRows - 1) / kSlabRows;
+  const int64_t each = ((p.I + slabs - 1) / slabs + 255) / 256 * 256;
+  int64_t sums = 0;
+  for (int64_t at = 0; at < p.I; at += each) {
+    ProductArgs q = p;
+    int64_t rows = 0;
+    q.I = p.I - at < each ? p.I - at : each;
+    q.a = (const T*)p.a + at * p.a_i;
+    q.extra = p.extra ? (const T*)p.extra + at * p.extra_row : nullptr;
+    q.out = (T*)p.out + at * p.out_row;
+    q.part_sum = p.part_sum ? p.part_sum + sums * width : nullptr;
+    q.sum_rows = &rows;
+    if (int rc = f(q)) return rc;
+    sums += rows;
+  }
+  if (p.sum_rows) *p.sum_rows = sums;
+  return 0;
+}
+
 template <typename T, bool RCA, bool RCB, int EPI, bool GATED, bool DIRECT, int BI, int WI, int BJ, int WJ>
 int launch_tiles(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   constexpr int kOut = GATED ? BJ / 2 : BJ;
   const int64_t ti = (p.I + BI - 1) / BI, tj = (p.J + kOut - 1) / kOut;
   if (ti > 0x7fffffff / tj || ti * tj > 0x7ffffff0 / splits) return 1;
   const int64_t total = ti * tj * splits, grid = (total + 7) / 8 * 8;
+  if (grid > kMostThreads / (64 * WI * WJ)) return 1;
   if (kColumnSums<T, EPI> && p.part_sum) *p.sum_rows = ti * WI;
   hipLaunchKernelGGL((product_kernel<T, RCA, RCB, EPI, GATED, DIRECT, BI, WI, BJ, WJ>), dim3((uint32_t)grid),
                      dim3(64 * WI * WJ), 0, stream, p, (uint32_t)ti, (uint32_t)tj, (uint32_t)splits);

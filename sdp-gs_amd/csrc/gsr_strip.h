@@ -294,7 +294,7 @@ int launch_strip(const ProductArgs& p, char* scratch, hipStream_t stream) {
   const int64_t part_tiles = (tiles + parts - 1) / parts;
   parts = (tiles + part_tiles - 1) / part_tiles;
   const int64_t items = strips * parts;
-  if (items > 0x7ffffff0 || chunks > 0x7fffffff) return 1;
+  if (items + 7 > kMostThreads / (64 * S::kWaves) || chunks > 0x7fffffff) return 1;
   if (kColumnSums<T, EPI> && p.part_sum) *p.sum_rows = strips * S::kWaves;
   // one small tile of weights is made by every workgroup itself: cheaper than a launch before this
   // one (762048x3x64 in 32 bits: 67 us a call with it, 57 without); not a large one (bf16
@@ -382,13 +382,17 @@ int dx_product(const ProductArgs& p, char* scratch, hipStream_t s) {
     return cut_bytes<T>(M, K, N, segments, false);                                                      \
   }                                                                                                  \
   template <> int product_forward<T>(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) { \
-    return forward_or_dz<T, EPI_FORWARD>(p, gated, scratch, s);                                      \
+    return in_slabs<T>(p, 0, [&](const ProductArgs& q) {                                             \
+      return forward_or_dz<T, EPI_FORWARD>(q, gated, scratch, s);                                    \
+    });                                                                                              \
   }                                                                                                  \
   template <> int product_dz<T>(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) {    \
-    return forward_or_dz<T, EPI_DZ>(p, gated, scratch, s);                                           \
+    return in_slabs<T>(p, gated ? 2 * p.J : p.J, [&](const ProductArgs& q) {                         \
+      return forward_or_dz<T, EPI_DZ>(q, gated, scratch, s);                                         \
+    });                                                                                              \
   }                                                                                                  \
   template <> int product_dx<T>(const ProductArgs& p, char* scratch, hipStream_t s) {                \
-    return dx_product<T>(p, scratch, s);                                                             \
+    return in_slabs<T>(p, 0, [&](const ProductArgs& q) { return dx_product<T>(q, scratch, s); });    \
   }                                                                                                  \
   template <> bool product_dw_huge<T>(const ProductArgs& p) {                                        \
     return sizeof(T) == 2 && takes_huge_dw(p.I, p.J) &&                                              \
