@@ -105,7 +105,7 @@ __device__ __forceinline__ float act_both(float z, float& value) {
     return s * fmaf(z, 1.0f - s, 1.0f);
   }
   value = act_value<ACT>(z);
-  if constexpr (ACT == GSR_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if constexpr (ACT == GSR_ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;  // 1 at NaN: the gradient goes through
   return 1.0f;
 }
 
