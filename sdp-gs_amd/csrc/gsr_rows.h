@@ -124,16 +124,21 @@ int launch_rows(const ProductArgs& p, hipStream_t s) {
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 
-// Where the tiled kernel has too few tiles (of 64 x 64) to go around.  us, these : tiles, bf16
-// 64x4096x4096 (64 tiles) 22 : 36, 128x4096x4096 (128) 39 : 36, 64x1024x6144 (96) 12 : 9,
-// 32x1024x6144 (96) 8.2 : 9.1, gated 16x2048x5504 17 : 22, 64x2048x5504 28 : 23; fp32
-// 128x4096x4096 (128) 84 : 104, 128x1024x6144 (192) 35 : 30, 64x1024x6144 (96) 24 : 28.
-template <typename T>
-bool rows_sizes(int64_t I, int64_t J, bool gated) {
+// Where this kernel is faster than the tiled one, whole or with its sum cut into ranges: where a wave's
+// own part of the sum is short -- R (1 + blocks of 16 rows) elements come in for each workgroup of 16
+// outputs, more than 256 workgroups take turns -- or where the weights of a single block of rows
+// stream through every CU.  us, these : tiled, bf16 64x1024x1024 7.6 : 9.2, 256x512x512 5.5 : 6.3,
+// 1x4096x4096 7.6 : 10.1, gated 16x2048x5504 14.2 : 14.9, but 64x4096x1024 20.6 : 9.1, 32x4096x4096
+// 14.1 : 11.7, 128x256x8192 10.5 : 5.2; fp32 64x512x512 8.2 : 11.5, 16x4096x4096 21.3 : 24.7, but
+// 64x8192x1024 79.7 : 17.6, 64x1024x6144 24.3 : 18.2.  Of 848 sizes (1 to 256 rows, 256 to 8192
+// inputs and outputs) the rule is 0.8 % off the faster one on average, at worst 1.44 times (fp32,
+// gated 1x4096x8192 95.5 : 66.1).
+inline bool rows_sizes(int64_t I, int64_t J, int64_t R) {
   if (I > 256) return false;
-  const int64_t tiles = (I + 63) / 64 * ((J + 63) / 64);
-  if (sizeof(T) == 4) return I <= 64 || tiles <= 128;
-  return I <= 32 || (I <= 64 && tiles <= 64 && !gated);
+  const int64_t blocks = I > 64 ? 4 : (I + 15) / 16, groups = (J + 15) / 16 * ((I + 63) / 64);
+  if (groups >= 256 && blocks == 1) return true;
+  if (groups > 256 && I > 64) return false;
+  return R * (1 + blocks) * (groups > 256 ? groups : 256) <= 5120 * 256;
 }
 
 }  // namespace gsr

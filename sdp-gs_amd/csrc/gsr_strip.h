@@ -345,12 +345,12 @@ size_t strips_scratch(int64_t J, int64_t R, bool gated) {
 template <typename T, int EPI>
 size_t forward_or_dz_scratch(int64_t M, int64_t K, int64_t N, bool gated) {
   if (takes_strips(M, K)) return strips_scratch<T>(N, K, gated);
-  return EPI == EPI_FORWARD && rows_sizes<T>(M, N, gated) ? 0 : cut_bytes<T>(M, N, K, 1, gated);
+  return EPI == EPI_FORWARD && rows_sizes(M, N, K) ? 0 : cut_bytes<T>(M, N, K, 1, gated);
 }
 
 template <typename T, int EPI>
 int forward_or_dz(const ProductArgs& p, bool gated, char* scratch, hipStream_t s) {
-  const bool strips = takes_strips(p.I, p.R), few = EPI == EPI_FORWARD && rows_sizes<T>(p.I, p.J, gated);
+  const bool strips = takes_strips(p.I, p.R), few = EPI == EPI_FORWARD && rows_sizes(p.I, p.J, p.R);
   if constexpr (EPI == EPI_FORWARD)
     if (few && p.a_r == 1) return gated ? launch_rows<T, EPI, true>(p, s) : launch_rows<T, EPI, false>(p, s);
   const int64_t cuts = strips || few || p.a_r != 1 ? 1 : cuts_of<T>(p.I, p.J, p.R, 1);

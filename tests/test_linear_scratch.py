@@ -48,3 +48,15 @@ def test_gradients_of_no_rows_and_wide_layers(kind, pair):
         y = gated_linear(x, w, u, b) if pair else fused_linear(x, w, b, activation="gelu")
         dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
         assert dx.shape == (0, K) and not bool(dw.any()) and not bool(db.any())
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_which_sums_of_few_rows_are_cut(kind):
+    """Ranges of a long sum need scratch memory: few outputs of a long sum are cut, weights that stream
+    past one block of rows, and short sums, are not."""
+    L = _lib.load()
+    for size in (L.gsr_linear_scratch_bytes, L.gsr_gated_scratch_bytes):
+        for M, K, N in ((64, 4096, 512), (64, 4096, 1024), (128, 8192, 1024), (17, 8192, 1000)):
+            assert size(kind, M, K, N) > 0, (M, K, N)
+        for M, K, N in ((1, 4096, 8192), (16, 2048, 5504), (5, 512, 512), (64, 1024, 1024), (256, 512, 512)):
+            assert size(kind, M, K, N) == 0, (M, K, N)
