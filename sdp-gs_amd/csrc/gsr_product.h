@@ -785,6 +785,7 @@ inline bool takes_huge_dw(int64_t I, int64_t J) { return I > 128 && J > 128; }  
 // : 128 x 128; bf16 512x4096x4096 43 : 52, 2048x512x512 7.1 : 10.4, fp32 17 : 34; at 1024x4096x4096,
 // 256 tiles, bf16 55 : 55, fp32 296 : 257).  128 x 64 for up to 64 columns of many rows (fp32
 // weight gradient of 762048x64x256 271, with 64 x 64 348; but of 762048x3x64, 64 rows, 128 : 76).
+// The 128 x 128 weight gradient in 32 bits keeps 7 registers in scratch memory.
 template <typename T, bool RCA, bool RCB, int EPI>
 int launch_linear(const ProductArgs& p, int64_t splits, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {

@@ -10,8 +10,16 @@
 // tile's results leave as soon as they are there.
 //
 // What bounds it: a view's layer 762048x256x512 in bfloat16 moves 1.17 GB (230 us at a copy's rate)
-// and takes 345 us forward; its products and its stores overlap only in part (156 us of the one and
-// 172 us of the other and of x's loads when timed alone).  762048x3x64 in 32 bits takes 55 us, 204 MB at 3.7 TB/s.
+// and takes 353 us forward, 380 with gelu (a call; its kernel alone 361 and more where x is not in a
+// cache); its products and its stores overlap only in part (156 us of the one and 172 us of the other
+// and of x's loads when timed alone).  762048x3x64 in 32 bits, channel-major, takes 57 us a call and
+// its kernel 49, 204 MB at 4.2 TB/s: each of the 5954 workgroups has a single tile, whose loads,
+// image, product and stores follow each other, and only the two others on its CU fill the gaps.
+//
+// Registers: three forms in 32 bits do not fit theirs and keep some in scratch memory, up to 32
+// inputs with a residual (48) or an incoming gradient (32), and 65 to 128 inputs (18 and 12).  It
+// shows little: with a residual, 762048x20x64 119 us (3.8 TB/s) and 762048x100x64 170 (4.1), forms
+// that fit 762048x60x64 136 (4.2) and 762048x160x64 233 (3.8).
 #pragma once
 #include "gsr_rows.h"
 
