@@ -128,8 +128,9 @@ def grad_norm(tensors, norm_type=2.0):
 
 
 def _refuse_overlap(c):
-    """Two workgroups may not scale the same memory.  Gradients with gaps are scaled in copies, so
-    only their overlap with one that is scaled in place counts."""
+    """Two workgroups may not scale the same memory.  Gradients with gaps are scaled in copies and may
+    lie between each other (columns of one buffer); refused are one that lies over a gradient that is
+    scaled in place, and two that begin at the same element."""
     if all(map(operator.is_, c.given, c.tensors)):
         spans = sorted(zip(c.pointers, c.ends))
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
@@ -144,10 +145,11 @@ def _refuse_overlap(c):
             start, end = t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
         spans.append((start, end, t is own))
     spans.sort()
-    end_dense = end_any = 0
+    end_dense = end_any = last = 0
     for start, end, dense in spans:
-        if start < (end_any if dense else end_dense):
+        if start < (end_any if dense else end_dense) or start == last:
             raise ValueError("clip_grad_norm_: two gradients share memory (the same one twice?)")
+        last = start
         if end > end_any:
             end_any = end
         if dense and end > end_dense:

@@ -57,6 +57,32 @@ def test_a_bad_limit_moves_nothing(bad):
     assert bool((p == 1).all()) and len(opt.state[p]) == 0
 
 
+@gpu
+def test_the_same_gradient_with_gaps_twice_is_refused():
+    """Columns of one buffer are clipped side by side, the same ones twice are not."""
+    from gsr_amd.optim import clip_grad_norm_
+    wide = torch.randn(30, 20, device="cuda")
+    keep = wide.clone()
+
+    def clip(*columns):
+        ps = []
+        for a, b in columns:
+            p = torch.nn.Parameter(torch.zeros(30, b - a, device="cuda"))
+            p.grad = wide[:, a:b]
+            ps.append(p)
+        return clip_grad_norm_(ps, 1e-3)
+
+    for columns in (((3, 10), (3, 10)), ((3, 10), (3, 8)), ((0, 2), (3, 10), (12, 14), (3, 10))):
+        with pytest.raises(ValueError, match="share memory"):
+            clip(*columns)
+    assert torch.equal(wide, keep)
+    norm = clip((3, 10), (0, 3), (12, 20))
+    c = 1e-3 / (float(norm) + 1e-6)
+    torch.testing.assert_close(wide[:, :10], keep[:, :10] * c, rtol=6 * 2 ** -24, atol=0)
+    torch.testing.assert_close(wide[:, 12:], keep[:, 12:] * c, rtol=6 * 2 ** -24, atol=0)
+    assert torch.equal(wide[:, 10:12], keep[:, 10:12])
+
+
 def test_c_entry_refuses_a_factor_from_a_bad_limit():
     """Status 1 before any GPU work where a factor is asked for; a norm alone has no limit."""
     from gsr_amd import _lib
