@@ -148,7 +148,7 @@ def train_iteration(model, cam, gt_image, depth_mono, bg, args: OptArgs, iterati
     from gaussian_renderer import render
     if (feature_head is None) != (gt_feature is None):
         raise ValueError("train_iteration: feature_head and gt_feature belong together")
-    if feature_head is not None:
+    if hasattr(feature_head, "refuse_training"):  # another module with its FusedAdam may stand in
         feature_head.refuse_training()
     pipe = pipe or _Pipe()
     pkg = render(cam, model, pipe, bg, args)

@@ -123,3 +123,29 @@ def test_the_norm_of_a_step_with_a_head_is_that_of_both():
     model.optimizer.max_grad_norm = None
     trainer._optimizer_step(model, args=trainer.OptArgs())
     assert model.optimizer.grad_norm is None
+
+
+class _PixelHead(_Head):
+    """A module of one's own that is called like a FeatureHead and has its optimizer."""
+
+    def forward(self, image, pixels=None):
+        rows = image.reshape(3, -1).t()
+        rows = super().forward(rows if pixels is None else rows[pixels])
+        return rows if pixels is not None else rows.reshape(image.shape[1], image.shape[2], 2)
+
+
+@gpu
+def test_a_module_of_ones_own_as_the_head():
+    from gsr_amd.model import SplatModel
+    from gsr_amd.synthetic import make_cameras, make_gaussians, training_targets
+    m = SplatModel(make_gaussians(500, sh_degree=3, seed=3), device="cuda")
+    cam = make_cameras(1, 64, 48, seed=3)[0].to("cuda")
+    gts, monos = training_targets(1, 48, 64, seed=2, device="cuda")
+    args = trainer.OptArgs()
+    trainer.make_trainable(m, args)
+    head = _PixelHead("cuda", None)
+    before = [p.detach().clone() for p in head.parameters()]
+    target = torch.randn(48, 64, 2, device="cuda")
+    trainer.train_iteration(m, cam, gts[0], monos[0], torch.zeros(3, device="cuda"), args, 1, 2.78,
+                            feature_head=head, gt_feature=target)
+    assert not any(torch.equal(a, p) for a, p in zip(before, head.parameters()))
