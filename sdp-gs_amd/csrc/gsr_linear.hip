@@ -100,8 +100,9 @@ struct ColumnSums {
 // what is returned in `sums`; `scratch` moves on behind what is kept.
 // 16-bit gradients are rounded once more here, the results of dx and dw have an error of 2.35e-3 in
 // bfloat16 where the one rounding of a result gives 1.66e-3: the matrix instruction takes operands of
-// one type, so more bits would be a second operand of remainders, written, read twice and multiplied
-// (of 762048x256x512, 2.3 GB and 0.4 TFLOP on top of 3.0 GB and 0.6 in these three passes).
+// one type, so more bits would be a second operand of remainders, written, read twice and multiplied.
+// That is what a pair's backward does with its second half: 2011 us for 762048x256x512 where a
+// layer's takes 1163.
 template <typename T>
 int activation_gradients(ProductArgs p, bool gated, bool need_db, char*& scratch, const float** sums,
                          int64_t* sum_rows, hipStream_t stream) {
